@@ -97,6 +97,106 @@ int s1_gdn_conv_gates_batch(const void* qkv, int ld, const void* w, void* q, voi
                             const int* len, int nseq, int key_dim, int value_dim, const void* b, const void* a,
                             const void* A_log, const void* dt_bias, void* beta, float* g, int H, void* stream);
 
+/* ---- The tokens after a prefill: the decode forms of the operators that carry state ----
+ * No counterpart in the reference, which only prefills. Float32 inside and one rounding at the end
+ * (the prefill's operators also round in between, where the model stores a tensor: a step's bf16
+ * results differ from theirs by a step of bf16 at times). Everything that changes from step to step
+ * (slots, positions, lengths, page tables) is int32 in device memory, so a recorded step replays with
+ * new contents; the kernels check every index before they use it. What they refuse they leave
+ * unwritten, with a code in the family's device error word (s1_device_status): 60 rows outside the
+ * operands, 61 a slot outside the pool, 62 sequences that would race for a slot (delta-rule family);
+ * 31 a row whose sequence or position the table does not have, 32 a page outside the pools, 33 a
+ * position outside the rotary tables, 34 rows at one place of the cache (attention family).
+ * The first call of an operator on a GPU looks up the address of that word: make it before any
+ * stream capture. All pointers belong to the current device, as everywhere in this interface. */
+
+/* Gated delta rule token by token: cs1_gdn_prefill_x for windows of a few tokens of many sequences, one
+ * launch. Sequence i owns rows [start[i], start[i + 1]) of q, k [rows, HK, 128], v, o [rows, H, 128], g
+ * and beta [rows, H] (start [nseq + 1], rows in ascending order; null: row i alone), begins with the
+ * state slot_in[i] (negative: zeros) and leaves its state in slot_out[i] (negative: the sequence sits
+ * out, its rows of o are left as they are). states: float32 [n_slots], slot_stride floats apart (a multiple of
+ * 4, at least H * 128 * 128), each [H, 128 (key), 128 (value)] as s_in / s_out there. slot_in[i] may equal slot_out[i]
+ * (update in place) and several sequences may begin with one slot that none of them writes (the
+ * candidates of a prefix); a slot that one sequence writes and another one names is refused for
+ * both. A sequence without rows copies its state. Float32 throughout. */
+int s1_gdn_step(const void* q, const void* k, const void* v, const float* g, const void* beta, void* o, int rows, int H,
+                int HK, float scale, float* states, int n_slots, size_t slot_stride, const int* start, const int* slot_in,
+                const int* slot_out, int nseq, void* stream);
+
+/* The convolution and gates before it: s1_gdn_conv_gates for rows that continue sequences. Rows,
+ * start, slots and their rules as in s1_gdn_step; a slot of tails (bf16, slot_stride elements apart, a multiple
+ * of 8, at least 3 * channels, channels = 2 * key_dim + value_dim) holds a sequence's last three rows of
+ * qkv [3, channels] before the convolution, the oldest first, zeros where it has fewer. key_dim, value_dim and ld
+ * multiples of 8; pointers but b, a, A_log, dt_bias, beta and g 16-byte aligned. At most 65535 sequences. */
+int s1_gdn_conv_gates_step(const void* qkv, int ld, const void* w, void* q, void* k, void* v, int rows, int key_dim,
+                           int value_dim, const void* b, const void* a, const void* A_log, const void* dt_bias, void* beta,
+                           float* g, int H, void* tails, int n_slots, size_t slot_stride, const int* start,
+                           const int* slot_in, const int* slot_out, int nseq, void* stream);
+
+/* A paged cache of one full-attention layer: two pools [n_pages, page_tokens, Hk, Dh] (keys after norm
+ * and rotary, values as projected; a captured prefix's keys are such a pool where page_tokens divides
+ * its length) and a table [n_seqs, table_pages] of page numbers: token p of sequence s is row
+ * p % page_tokens of page table[s][p / page_tokens]. Entries behind a sequence's last page are never
+ * read; sequences may share pages. n_pages * page_tokens < 2^31, table_pages * page_tokens <= 2^30.
+ *
+ * cs1_attn_prep for rows anywhere in such a cache: row r is token pos[r] of sequence seq[r] (seq null:
+ * sequence r; pos negative: the row sits out). qg [rows, Hq, 2 * Dh], kr and vr [rows, Hk, Dh] lie in
+ * rows of ld elements; q and gate [rows, Hq, Dh] come out, keys and values go to their places in the cache. The rotary
+ * tables cos, sin [angles, half] are read at row angle[r] (null: at pos[r]), so tables of one row per
+ * packed row serve positions on several axes. Rows at one place of the cache are refused: their q
+ * and gate come out, the place is left as it is. Any page_tokens; 16-byte aligned pointers. */
+int s1_attn_prep_paged(const void* qg, const void* kr, const void* vr, int ld, const void* qw, const void* kw,
+                       const void* cos, const void* sin, int angles, const int* angle, void* q, void* gate, void* k_pages,
+                       void* v_pages, int n_pages, int page_tokens, const int* table, int table_pages, int n_seqs,
+                       const int* seq, const int* pos, int rows, int Hq, int Hk, int Dh, int half, float eps, void* stream);
+
+/* Attention of one new token per row: q, out [rows, Hq, Dh], row r over the first len[r] tokens of
+ * sequence seq[r] (null: r), its own one among them; several rows of one sequence with growing len
+ * are a causal window. gate (nullable) [rows, Hq, Dh]: out = o * sigmoid(gate). len 0: zeros; len
+ * negative: the row sits out, out is left as it is. A row with a page outside the pools comes out
+ * undefined (code 32), a row that the table does not have is left as it is (code 31); a row whose scores are all -inf comes out
+ * as zeros. page_tokens a multiple of 16, Dh 128 or 256, Hq a multiple of Hk, at most 2^20 rows; pools
+ * and workspace 16-byte aligned, q, gate and out 4. Two launches; the result does not depend on
+ * what else runs, only on the lengths of the call (they decide where the cache is cut). The workspace (at least
+ * s1_attention_paged_workspace_floats; 0 for shapes that the operator does not take) needs no
+ * clearing and belongs to one call at a time. */
+size_t s1_attention_paged_workspace_floats(int Hq, int Hk, int Dh);
+int s1_attention_paged(const void* q, const void* gate, void* out, const void* k_pages, const void* v_pages, int n_pages,
+                       int page_tokens, const int* table, int table_pages, int n_seqs, const int* seq, const int* len,
+                       int rows, int Hq, int Hk, int Dh, float scale, float* workspace, size_t workspace_floats,
+                       void* stream);
+
+/* Copies whole pages: page dst[i] becomes page src[i], i < n, in each of n_pools pools [n_pages] of
+ * page_bytes bytes a page (a multiple of 16; pools 16-byte aligned). pools, src and dst are host
+ * arrays and may change as soon as the call returns; a recorded call keeps its lists. Several
+ * destinations may share a source. S1_ERR_ARGUMENT-like refusals are cudaErrorInvalidValue: a page
+ * out of range, twice among the destinations, or both a source and a destination. Slots of s1_gdn_step and
+ * s1_gdn_conv_gates_step are pages as well (page_bytes = their stride). */
+int s1_pages_copy(void* const* pools, int n_pools, int n_pages, size_t page_bytes, const int* src, const int* dst, int n,
+                  void* stream);
+
+/* Who owns which page: the host's side of the tables (no device memory, no GPU needed; one thread
+ * at a time per handle). Sequences are numbers below max_seqs, empty at first. A call that fails
+ * changes nothing. Copies that a call asks for go into src and dst (room for `cap`; null with cap 0)
+ * and have to run (s1_pages_copy, on the stream of the operators) before the next step. */
+int s1_pages_create(int n_pages, int page_tokens, int max_seqs, int max_seq_pages, void** pages);
+void s1_pages_destroy(void* pages);
+/* Room for `tokens` more tokens at the sequence's end. New tokens must not land in a page that another
+ * sequence names: a shared, partly filled last page is replaced by a copy (at most one copy per call).
+ * S1_ERR_PAGES when free pages, the sequence's table row or `cap` do not suffice. */
+int s1_pages_append(void* pages, int seq, int tokens, int* src, int* dst, int cap, int* n_copies);
+/* The empty sequence `to` becomes a second name of `from`'s pages. */
+int s1_pages_fork(void* pages, int from, int to);
+/* Drops the tokens behind the first `tokens` (0 frees the sequence); pages that no sequence names
+ * any more are free again. */
+int s1_pages_truncate(void* pages, int seq, int tokens);
+/* Moves pages so that the used ones are the first of the pools. */
+int s1_pages_compact(void* pages, int* src, int* dst, int cap, int* n_copies);
+/* Page numbers of sequences [seq, seq + n) into table [n, table_pages], -1 behind the last, and
+ * their tokens into len (each nullable). S1_ERR_ARGUMENT where a row is too short for a sequence. */
+int s1_pages_table(void* pages, int seq, int n, int* table, int table_pages, int* len);
+int s1_pages_free_count(void* pages);
+
 /* The attention kernel's counterpart of s1_gemm_tc5_status: its device error word (0 = no bounded
  * wait ever gave up), read after waiting for all queued work, then cleared. */
 int s1_attn_tc5_status(int* code);
@@ -331,6 +431,7 @@ int s1_assign_requests_weighted(const int* lengths, int n, int n_ranks, double a
 #define S1_ERR_CHECKPOINT_DTYPE 3006   /* a language-model tensor is not bfloat16 (model.rs:291-295) */
 #define S1_ERR_CHECKPOINT_MISSING 3007 /* no embed_tokens.weight, or a tensor of the decoder is absent */
 #define S1_ERR_EXPORT_FIELD 3008       /* open_jev_export.json lacks a field or holds an invalid value */
+#define S1_ERR_PAGES 3009              /* not enough free pages, table room or list room */
 
 #ifdef __cplusplus
 }

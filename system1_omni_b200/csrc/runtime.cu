@@ -15,7 +15,7 @@ const char* cs1_error_string(int code) {
     if (code >= CS1_ERR_GEMM_BASE && code < CS1_ERR_UNSUPPORTED) return "GEMM handle or engine error (code - 1000)";
     switch (code) {
         case CS1_ERR_UNSUPPORTED: return "operation not built into this library";
-        case CS1_ERR_DEVICE_CHECK: return "a device-side bounded wait gave up";
+        case CS1_ERR_DEVICE_CHECK: return "a device-side bounded wait gave up, or a step operator refused an index";
         case CS1_ERR_TENSOR_MAP: return "TMA tensor map encoding failed";
         case CS1_ERR_STATIC_SCRATCH: return "window larger than the fixed scratch of cs1_gdn_prefill_static";
         case 3000: return "executor: invalid argument";
@@ -27,6 +27,7 @@ const char* cs1_error_string(int code) {
         case 3006: return "checkpoint: tensor is not bfloat16";
         case 3007: return "checkpoint: embed_tokens.weight or a tensor of the decoder is missing";
         case 3008: return "export manifest: a field is missing or invalid";
+        case 3009: return "pages: not enough free pages, table room or list room";
         case 3100: return "dispatcher: libnccl.so.2 cannot be loaded";
         case 3101: return "dispatcher: the communicator id could not be exchanged";
         case 3102: return "dispatcher: an NCCL call failed";

@@ -1,0 +1,283 @@
+// The Gated DeltaNet operators of the tokens after a prefill: the convolution and the gates of new
+// rows behind kept ones, and the gated delta rule token by token.
+//
+// Float32 from the inputs to one rounding at the end. The prefill's operators round in between where
+// the model stores a tensor (the convolution before its SiLU), so a step's bf16 results differ from
+// theirs by a step of bf16 at times; what a slot keeps is the same.
+#include "cs1_ops.h"
+#include "s1_executor.h"
+#include "status.h"
+#include "step.h"
+
+namespace s1 {
+namespace {
+
+constexpr int D = 128;  // key and value dim of the delta rule
+
+// ---- delta rule ----
+// Per token, with k = k/|k|, q = scale q/|q| (both with 1e-6 under the root) and the state S [key, value]:
+//   d = beta (v - e^g k^T S),  S <- e^g S + k d^T,  o = q^T S = e^g q^T S_before + (q.k) d.
+// The value columns are independent of one another, so a warp takes CW of them with all 128 keys and
+// keeps its part of S in registers over the window's tokens: S is read once and written once, and
+// both products of a token come from one pass over the registers. Lane l owns columns
+// 4 (l % (CW/4)) .. + 3 of the keys l / (CW/4), + RG, ...; the sums over keys are closed by shuffles.
+template <int CW>
+__global__ void __launch_bounds__(128)
+    gdn_step_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
+                    const float* __restrict__ g, const bf16* __restrict__ beta, bf16* __restrict__ o, int H, int group,
+                    float scale, float* states, size_t slot_stride, const StepSeqs seqs, int* error) {
+    constexpr int CL = CW / 4, RG = 32 / CL, RL = D / RG;  // lanes over columns, groups of lanes over keys, keys per lane
+    constexpr int PARTS = D / CW;
+    __shared__ float2 kq_all[4][D];
+    grid_dep_trigger();
+    grid_dep_sync();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long unit = (long long)blockIdx.x * 4 + warp;
+    const int part = (int)(unit % PARTS), h = (int)(unit / PARTS % H);
+    const int i = (int)(unit / PARTS / H);
+    if (i >= seqs.nseq) return;
+    const StepSeq sq = step_sequence(seqs, i);
+    if (sq.code && lane == 0) atomicCAS(error, 0, sq.code);
+    if (sq.rows < 0) return;
+    const int c0 = part * CW + lane % CL * 4, r0 = lane / CL;
+    float2* kq = kq_all[warp];
+
+    float4 S[RL];
+    if (sq.in >= 0) {
+        const float* src = states + (size_t)sq.in * slot_stride + ((size_t)h * D + r0) * D + c0;
+#pragma unroll
+        for (int j = 0; j < RL; j++) S[j] = *reinterpret_cast<const float4*>(src + (size_t)j * RG * D);
+    } else {
+#pragma unroll
+        for (int j = 0; j < RL; j++) S[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    if (__any_sync(0xffffffffu, step_clash(seqs, i, sq.in, sq.out, lane, 32))) {
+        if (lane == 0) atomicCAS(error, 0, STEP_SLOT_CLASH);
+        return;
+    }
+
+    const int hk = h / group, HK = H / group;
+    for (int t = 0; t < sq.rows; t++) {
+        const size_t row = (size_t)sq.row0 + t;
+        const uint2 kr = *reinterpret_cast<const uint2*>(k + (row * HK + hk) * D + lane * 4);
+        const uint2 qr = *reinterpret_cast<const uint2*>(q + (row * HK + hk) * D + lane * 4);
+        const uint2 vr = *reinterpret_cast<const uint2*>(v + (row * H + h) * D + c0);
+        const float decay = expf(g[row * H + h]), b = f32(beta[row * H + h]);
+        const float kv[4] = {__uint_as_float(kr.x << 16), __uint_as_float(kr.x & 0xffff0000u), __uint_as_float(kr.y << 16),
+                             __uint_as_float(kr.y & 0xffff0000u)};
+        const float qv[4] = {__uint_as_float(qr.x << 16), __uint_as_float(qr.x & 0xffff0000u), __uint_as_float(qr.y << 16),
+                             __uint_as_float(qr.y & 0xffff0000u)};
+        float kk = 0.f, qq = 0.f, qk = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) kk += kv[e] * kv[e], qq += qv[e] * qv[e], qk += kv[e] * qv[e];
+        kk = rsqrtf(warp_sum(kk) + 1e-6f);
+        qq = rsqrtf(warp_sum(qq) + 1e-6f) * scale;
+        qk = warp_sum(qk) * kk * qq;
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 4; e++) kq[lane * 4 + e] = make_float2(kv[e] * kk, qv[e] * qq);
+        __syncwarp();
+
+        float ks[4] = {}, qs[4] = {};
+#pragma unroll
+        for (int j = 0; j < RL; j++) {
+            const float2 c = kq[r0 + j * RG];
+            ks[0] += c.x * S[j].x, ks[1] += c.x * S[j].y, ks[2] += c.x * S[j].z, ks[3] += c.x * S[j].w;
+            qs[0] += c.y * S[j].x, qs[1] += c.y * S[j].y, qs[2] += c.y * S[j].z, qs[3] += c.y * S[j].w;
+        }
+#pragma unroll
+        for (int m = CL; m < 32; m <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                ks[e] += __shfl_xor_sync(0xffffffffu, ks[e], m);
+                qs[e] += __shfl_xor_sync(0xffffffffu, qs[e], m);
+            }
+        const float vv[4] = {__uint_as_float(vr.x << 16), __uint_as_float(vr.x & 0xffff0000u), __uint_as_float(vr.y << 16),
+                             __uint_as_float(vr.y & 0xffff0000u)};
+        float d[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            d[e] = b * (vv[e] - decay * ks[e]);
+            y[e] = decay * qs[e] + qk * d[e];
+        }
+        if (r0 == 0) {
+            uint2 p;
+            p.x = pack2(y[0], y[1]);
+            p.y = pack2(y[2], y[3]);
+            *reinterpret_cast<uint2*>(o + (row * H + h) * D + c0) = p;
+        }
+#pragma unroll
+        for (int j = 0; j < RL; j++) {
+            const float kc = kq[r0 + j * RG].x;
+            S[j].x = decay * S[j].x + kc * d[0];
+            S[j].y = decay * S[j].y + kc * d[1];
+            S[j].z = decay * S[j].z + kc * d[2];
+            S[j].w = decay * S[j].w + kc * d[3];
+        }
+    }
+    if (sq.rows == 0 && sq.in == sq.out) return;
+    float* dst = states + (size_t)sq.out * slot_stride + ((size_t)h * D + r0) * D + c0;
+#pragma unroll
+    for (int j = 0; j < RL; j++) *reinterpret_cast<float4*>(dst + (size_t)j * RG * D) = S[j];
+}
+
+// ---- convolution and gates ----
+// y_t = silu(sum_j w_j x_{t-3+j}) per channel, the rows before a sequence's first out of its slot's
+// tail [3, channels] (x_{-3}, x_{-2}, x_{-1}, before the convolution). A thread walks the window's rows
+// for 8 channels with the three rows before in registers; the last row of blocks computes the gates.
+constexpr int CONV_THREADS = 128;
+
+__global__ void __launch_bounds__(CONV_THREADS)
+    gdn_conv_gates_step_kernel(const bf16* __restrict__ qkv, int ld, const bf16* __restrict__ w, bf16* __restrict__ q,
+                               bf16* __restrict__ k, bf16* __restrict__ v, int key_dim, int value_dim, int conv_blocks,
+                               const bf16* __restrict__ b, const bf16* __restrict__ a, const bf16* __restrict__ A_log,
+                               const bf16* __restrict__ dt_bias, bf16* __restrict__ beta, float* __restrict__ g, int H,
+                               bf16* tails, size_t slot_stride, const StepSeqs seqs, int* error) {
+    grid_dep_trigger();
+    grid_dep_sync();
+    const int i = blockIdx.y;
+    const StepSeq sq = step_sequence(seqs, i);
+    if (sq.code && threadIdx.x == 0) atomicCAS(error, 0, sq.code);
+    if (sq.rows < 0) return;
+    const int channels = 2 * key_dim + value_dim;
+    const int c0 = ((int)blockIdx.x * CONV_THREADS + (int)threadIdx.x) * 8;
+    const bool conv = (int)blockIdx.x < conv_blocks && c0 < channels;
+    uint4 x[3] = {};
+    if (conv && sq.in >= 0) {
+        const bf16* src = tails + (size_t)sq.in * slot_stride + c0;
+#pragma unroll
+        for (int j = 0; j < 3; j++) x[j] = ld16(src + (size_t)j * channels);
+    }
+    if (__syncthreads_or(step_clash(seqs, i, sq.in, sq.out, threadIdx.x, CONV_THREADS))) {
+        if (threadIdx.x == 0) atomicCAS(error, 0, STEP_SLOT_CLASH);
+        return;
+    }
+    if ((int)blockIdx.x >= conv_blocks) {
+        for (int e = threadIdx.x; e < sq.rows * H; e += CONV_THREADS) {
+            const size_t row = (size_t)sq.row0 + e / H;
+            const int h = e % H;
+            beta[row * H + h] = to_bf16(sigmoid(f32(b[row * ld + h])));
+            const float z = f32(a[row * ld + h]) + f32(dt_bias[h]);
+            g[row * H + h] = -expf(f32(A_log[h])) * (z > 20.f ? z : log1pf(expf(z)));
+        }
+        return;
+    }
+    if (!conv) return;
+    float wf[8][4];
+    {
+        const bf16* wp = w + (size_t)c0 * 4;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float tmp[8];
+            unpack8(ld16(wp + j * 8), tmp);
+#pragma unroll
+            for (int e = 0; e < 8; e++) wf[(j * 8 + e) / 4][(j * 8 + e) % 4] = tmp[e];
+        }
+    }
+    bf16* dst;
+    int dld, dc;
+    if (c0 < key_dim)
+        dst = q, dld = key_dim, dc = c0;
+    else if (c0 < 2 * key_dim)
+        dst = k, dld = key_dim, dc = c0 - key_dim;
+    else
+        dst = v, dld = value_dim, dc = c0 - 2 * key_dim;
+    for (int t = 0; t < sq.rows; t++) {
+        const size_t row = (size_t)sq.row0 + t;
+        const uint4 now = ld16_stream(qkv + row * ld + c0);
+        float x0[8], x1[8], x2[8], x3[8], y[8];
+        unpack8(x[0], x0);
+        unpack8(x[1], x1);
+        unpack8(x[2], x2);
+        unpack8(now, x3);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float acc = wf[e][0] * x0[e];
+            acc = fmaf(wf[e][1], x1[e], acc);
+            acc = fmaf(wf[e][2], x2[e], acc);
+            acc = fmaf(wf[e][3], x3[e], acc);
+            y[e] = silu_fast(acc);
+        }
+        st16(dst + row * dld + dc, pack8(y));
+        x[0] = x[1];
+        x[1] = x[2];
+        x[2] = now;
+    }
+    bf16* keep = tails + (size_t)sq.out * slot_stride + c0;
+#pragma unroll
+    for (int j = 0; j < 3; j++) st16(keep + (size_t)j * channels, x[j]);
+}
+
+// The delta-rule family's error word on the current device, looked up once per device.
+int error_word(int** p) {
+    static int* address[64] = {};
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64) return cudaErrorInvalidDevice;
+    if (!address[dev]) {
+        int* a = nullptr;
+        const int rc = gdn_error_address(&a);
+        if (rc != 0) return rc;
+        address[dev] = a;
+    }
+    *p = address[dev];
+    return 0;
+}
+
+}  // namespace
+}  // namespace s1
+
+using namespace s1;
+
+extern "C" int s1_gdn_step(const void* q, const void* k, const void* v, const float* g, const void* beta, void* o, int rows,
+                           int H, int HK, float scale, float* states, int n_slots, size_t slot_stride, const int* start,
+                           const int* slot_in, const int* slot_out, int nseq, void* stream) {
+    const StepSeqs seqs{start, slot_in, slot_out, nseq, rows, n_slots};
+    if (!step_seqs_ok(seqs) || H <= 0 || HK <= 0 || H % HK != 0 || slot_stride < (size_t)H * D * D || slot_stride % 4 != 0)
+        return cudaErrorInvalidValue;
+    if (nseq == 0) return cudaSuccess;
+    if (!states || !aligned16(states)) return cudaErrorInvalidValue;
+    if (rows > 0 && (!q || !k || !v || !g || !beta || !o || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)))
+        return cudaErrorInvalidValue;
+    constexpr int CW = 32;
+    const long long units = (long long)nseq * H * (D / CW);
+    if (units > 0x7fffffffLL) return cudaErrorInvalidValue;
+    int* error = nullptr;
+    const int rc = error_word(&error);
+    if (rc != 0) return rc;
+    const cudaError_t e =
+        launch_dep(gdn_step_kernel<CW>, (unsigned)((units + 3) / 4), 128, 0, as_stream(stream), static_cast<const bf16*>(q),
+                   static_cast<const bf16*>(k), static_cast<const bf16*>(v), g, static_cast<const bf16*>(beta),
+                   static_cast<bf16*>(o), H, H / HK, scale, states, slot_stride, seqs, error);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+extern "C" int s1_gdn_conv_gates_step(const void* qkv, int ld, const void* w, void* q, void* k, void* v, int rows, int key_dim,
+                                      int value_dim, const void* b, const void* a, const void* A_log, const void* dt_bias,
+                                      void* beta, float* g, int H, void* tails, int n_slots, size_t slot_stride,
+                                      const int* start, const int* slot_in, const int* slot_out, int nseq, void* stream) {
+    const StepSeqs seqs{start, slot_in, slot_out, nseq, rows, n_slots};
+    if (!step_seqs_ok(seqs) || key_dim <= 0 || value_dim <= 0 || key_dim % 8 != 0 || value_dim % 8 != 0 || H <= 0 || ld % 8 != 0 ||
+        (long long)ld < 2LL * key_dim + value_dim || ld < H || 2LL * key_dim + value_dim > 0x7fffffffLL)
+        return cudaErrorInvalidValue;
+    const int channels = 2 * key_dim + value_dim;
+    if (slot_stride < 3 * (size_t)channels || slot_stride % 8 != 0 || (long long)rows * H > 0x7fffffffLL || nseq > 65535)
+        return cudaErrorInvalidValue;
+    if (nseq == 0) return cudaSuccess;
+    if (!tails || !aligned16(tails) || !w || !aligned16(w) || !A_log || !dt_bias) return cudaErrorInvalidValue;
+    if (rows > 0 && (!qkv || !q || !k || !v || !b || !a || !beta || !g || !aligned16(qkv) || !aligned16(q) || !aligned16(k) ||
+                     !aligned16(v)))
+        return cudaErrorInvalidValue;
+    int* error = nullptr;
+    const int rc = error_word(&error);
+    if (rc != 0) return rc;
+    const int conv_blocks = (channels / 8 + CONV_THREADS - 1) / CONV_THREADS;
+    const cudaError_t e = launch_dep(
+        gdn_conv_gates_step_kernel, dim3(conv_blocks + 1, nseq), CONV_THREADS, 0, as_stream(stream),
+        static_cast<const bf16*>(qkv), ld, static_cast<const bf16*>(w), static_cast<bf16*>(q), static_cast<bf16*>(k),
+        static_cast<bf16*>(v), key_dim, value_dim, conv_blocks, static_cast<const bf16*>(b), static_cast<const bf16*>(a),
+        static_cast<const bf16*>(A_log), static_cast<const bf16*>(dt_bias), static_cast<bf16*>(beta), g, H,
+        static_cast<bf16*>(tails), slot_stride, seqs, error);
+    return e != cudaSuccess ? e : cudaGetLastError();
+}

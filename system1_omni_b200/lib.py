@@ -139,6 +139,22 @@ SIGNATURES = {
     "s1_attn_prep_batch": (i32, [vp, vp, i32, vp, vp, vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, f32, vp]),
     "s1_attention_gated_batch": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, i32, i32, vp, vp, i32, i32, i32, i32, f32, vp]),
     "s1_gdn_prefill_batch": (i32, [vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp, vp, i32, i32, i32, f32, vp, vp, vp]),
+    "s1_gdn_step": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, f32, vp, i32, sz, vp, vp, vp, i32, vp]),
+    "s1_gdn_conv_gates_step": (i32, [vp, i32, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, vp, vp, i32, vp, i32, sz, vp, vp,
+                                     vp, i32, vp]),
+    "s1_attn_prep_paged": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, i32, i32, vp, i32, i32, vp, vp, i32,
+                                 i32, i32, i32, i32, f32, vp]),
+    "s1_attention_paged_workspace_floats": (sz, [i32, i32, i32]),
+    "s1_attention_paged": (i32, [vp, vp, vp, vp, vp, i32, i32, vp, i32, i32, vp, vp, i32, i32, i32, i32, f32, vp, sz, vp]),
+    "s1_pages_copy": (i32, [vp, i32, i32, sz, vp, vp, i32, vp]),
+    "s1_pages_create": (i32, [i32, i32, i32, i32, vpp]),
+    "s1_pages_destroy": (None, [vp]),
+    "s1_pages_append": (i32, [vp, i32, i32, vp, vp, i32, ip]),
+    "s1_pages_fork": (i32, [vp, i32, i32]),
+    "s1_pages_truncate": (i32, [vp, i32, i32]),
+    "s1_pages_compact": (i32, [vp, vp, vp, i32, ip]),
+    "s1_pages_table": (i32, [vp, i32, i32, vp, i32, vp]),
+    "s1_pages_free_count": (i32, [vp]),
     "s1_assign_requests_weighted": (i32, [vp, i32, i32, f64, f64, vp, vp]),
     "s1_device_status": (i32, [ip, ip, ip]),
     "s1_selftest_wait_runs_out": (i32, [i32, vp]),
