@@ -20,105 +20,160 @@ constexpr int D = 128;  // key and value dim of the delta rule
 // The value columns are independent of one another, so a warp takes CW of them with all 128 keys and
 // keeps its part of S in registers over the window's tokens: S is read once and written once, and
 // both products of a token come from one pass over the registers. Lane l owns columns
-// 4 (l % (CW/4)) .. + 3 of the keys l / (CW/4), + RG, ...; the sums over keys are closed by shuffles.
-template <int CW>
-__global__ void __launch_bounds__(128)
+// 4 (l % (CW/4)) .. + 3 of the keys l / (CW/4), + RG, ...; the sums over keys are closed by shuffles. The warps
+// of a (sequence, head) are one block and prepare the rows (norms, gates) of up to CHUNK tokens together.
+typedef unsigned long long f32x2;  // two floats, the unit of the packed FMA
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ f32x2 two(float lo, float hi) {
+    f32x2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void lds(uint32_t at, f32x2& a, f32x2& b) { asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a), "=l"(b) : "r"(at)); }
+// Volatile: the update reads the keys again rather than hold 64 registers of them from the products on.
+__device__ __forceinline__ f32x2 lds_again(uint32_t at) {
+    f32x2 a;
+    asm volatile("ld.volatile.shared.b64 %0, [%1];" : "=l"(a) : "r"(at));
+    return a;
+}
+__device__ __forceinline__ void split(f32x2 x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ void unpack4(uint2 p, float (&x)[4]) {
+    x[0] = __uint_as_float(p.x << 16), x[1] = __uint_as_float(p.x & 0xffff0000u);
+    x[2] = __uint_as_float(p.y << 16), x[3] = __uint_as_float(p.y & 0xffff0000u);
+}
+
+//
+// HBM bounds it with one token a sequence: 64 KiB of state in, 64 KiB out per head, all of a block's reads
+// issued at once. Measured at 193 sequences of 48 heads (1.22 GB): 187 us, 6.53 TB/s; columns per warp and
+// blocks per SM at least: 32 and 2: 189 us, 16 and 2: 228, 8 and 2: 276 (narrower warps fetch pieces of lines).
+constexpr int CW = 32, CHUNK = 8;
+
+__global__ void __launch_bounds__(D / CW * 32, 3)
     gdn_step_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
                     const float* __restrict__ g, const bf16* __restrict__ beta, bf16* __restrict__ o, int H, int group,
                     float scale, float* states, size_t slot_stride, const StepSeqs seqs, int* error) {
     constexpr int CL = CW / 4, RG = 32 / CL, RL = D / RG;  // lanes over columns, groups of lanes over keys, keys per lane
-    constexpr int PARTS = D / CW;
-    __shared__ float2 kq_all[4][D];
+    constexpr int WARPS = D / CW;
+    __shared__ __align__(16) float4 kkqq[CHUNK][D];  // k, k, q, q
+    __shared__ __align__(16) uint2 vs[CHUNK][D / 4];
+    __shared__ float4 gates[CHUNK];                  // e^g, beta, q.k
     grid_dep_trigger();
     grid_dep_sync();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * 4 + warp;
-    const int part = (int)(unit % PARTS), h = (int)(unit / PARTS % H);
-    const int i = (int)(unit / PARTS / H);
-    if (i >= seqs.nseq) return;
+    const int h = (int)(blockIdx.x % H), i = (int)(blockIdx.x / H);
     const StepSeq sq = step_sequence(seqs, i);
-    if (sq.code && lane == 0) atomicCAS(error, 0, sq.code);
+    if (sq.code && threadIdx.x == 0) atomicCAS(error, 0, sq.code);
     if (sq.rows < 0) return;
-    const int c0 = part * CW + lane % CL * 4, r0 = lane / CL;
-    float2* kq = kq_all[warp];
+    const int c0 = warp * CW + lane % CL * 4, r0 = lane / CL;
 
-    float4 S[RL];
+    ulonglong2 S[RL];
     if (sq.in >= 0) {
         const float* src = states + (size_t)sq.in * slot_stride + ((size_t)h * D + r0) * D + c0;
 #pragma unroll
-        for (int j = 0; j < RL; j++) S[j] = *reinterpret_cast<const float4*>(src + (size_t)j * RG * D);
+        for (int j = 0; j < RL; j++) S[j] = *reinterpret_cast<const ulonglong2*>(src + (size_t)j * RG * D);
     } else {
 #pragma unroll
-        for (int j = 0; j < RL; j++) S[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < RL; j++) S[j] = make_ulonglong2(0, 0);
     }
-    if (__any_sync(0xffffffffu, step_clash(seqs, i, sq.in, sq.out, lane, 32))) {
-        if (lane == 0) atomicCAS(error, 0, STEP_SLOT_CLASH);
+    const bool clash = step_clash(seqs, i, sq.in, sq.out, threadIdx.x, WARPS * 32);
+    if (sq.rows == 0 && __syncthreads_or(clash)) {
+        if (threadIdx.x == 0) atomicCAS(error, 0, STEP_SLOT_CLASH);
         return;
     }
 
     const int hk = h / group, HK = H / group;
-    for (int t = 0; t < sq.rows; t++) {
-        const size_t row = (size_t)sq.row0 + t;
-        const uint2 kr = *reinterpret_cast<const uint2*>(k + (row * HK + hk) * D + lane * 4);
-        const uint2 qr = *reinterpret_cast<const uint2*>(q + (row * HK + hk) * D + lane * 4);
-        const uint2 vr = *reinterpret_cast<const uint2*>(v + (row * H + h) * D + c0);
-        const float decay = expf(g[row * H + h]), b = f32(beta[row * H + h]);
-        const float kv[4] = {__uint_as_float(kr.x << 16), __uint_as_float(kr.x & 0xffff0000u), __uint_as_float(kr.y << 16),
-                             __uint_as_float(kr.y & 0xffff0000u)};
-        const float qv[4] = {__uint_as_float(qr.x << 16), __uint_as_float(qr.x & 0xffff0000u), __uint_as_float(qr.y << 16),
-                             __uint_as_float(qr.y & 0xffff0000u)};
-        float kk = 0.f, qq = 0.f, qk = 0.f;
+#pragma unroll 1
+    for (int t0 = 0; t0 < sq.rows; t0 += CHUNK) {
+        const int nt = min(CHUNK, sq.rows - t0);
+        if (t0 > 0) __syncthreads();  // the rows before have been read
+#pragma unroll 1
+        for (int t = warp; t < nt; t += WARPS) {
+            const size_t row = (size_t)sq.row0 + t0 + t;
+            const uint2 kr = *reinterpret_cast<const uint2*>(k + (row * HK + hk) * D + lane * 4);
+            const uint2 qr = *reinterpret_cast<const uint2*>(q + (row * HK + hk) * D + lane * 4);
+            vs[t][lane] = *reinterpret_cast<const uint2*>(v + (row * H + h) * D + lane * 4);
+            const float gt = g[row * H + h], bt = f32(beta[row * H + h]);
+            float kv[4], qv[4];
+            unpack4(kr, kv);
+            unpack4(qr, qv);
+            float kk = 0.f, qq = 0.f, qk = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) kk += kv[e] * kv[e], qq += qv[e] * qv[e], qk += kv[e] * qv[e];
-        kk = rsqrtf(warp_sum(kk) + 1e-6f);
-        qq = rsqrtf(warp_sum(qq) + 1e-6f) * scale;
-        qk = warp_sum(qk) * kk * qq;
-        __syncwarp();
+            for (int e = 0; e < 4; e++) kk += kv[e] * kv[e], qq += qv[e] * qv[e], qk += kv[e] * qv[e];
+            kk = rsqrtf(warp_sum(kk) + 1e-6f);
+            qq = rsqrtf(warp_sum(qq) + 1e-6f) * scale;
+            qk = warp_sum(qk) * kk * qq;
 #pragma unroll
-        for (int e = 0; e < 4; e++) kq[lane * 4 + e] = make_float2(kv[e] * kk, qv[e] * qq);
-        __syncwarp();
-
-        float ks[4] = {}, qs[4] = {};
-#pragma unroll
-        for (int j = 0; j < RL; j++) {
-            const float2 c = kq[r0 + j * RG];
-            ks[0] += c.x * S[j].x, ks[1] += c.x * S[j].y, ks[2] += c.x * S[j].z, ks[3] += c.x * S[j].w;
-            qs[0] += c.y * S[j].x, qs[1] += c.y * S[j].y, qs[2] += c.y * S[j].z, qs[3] += c.y * S[j].w;
+            for (int e = 0; e < 4; e++) kkqq[t][lane * 4 + e] = make_float4(kv[e] * kk, kv[e] * kk, qv[e] * qq, qv[e] * qq);
+            if (lane == 0) gates[t] = make_float4(expf(gt), bt, qk, 0.f);
         }
+        if (t0 == 0) {
+            if (__syncthreads_or(clash)) {
+                if (threadIdx.x == 0) atomicCAS(error, 0, STEP_SLOT_CLASH);
+                return;
+            }
+        } else {
+            __syncthreads();
+        }
+#pragma unroll 1
+        for (int t = 0; t < nt; t++) {
+            const uint32_t rows_at = (uint32_t)__cvta_generic_to_shared(&kkqq[t][r0]);
+            f32x2 k01 = 0, k23 = 0, q01 = 0, q23 = 0;
 #pragma unroll
-        for (int m = CL; m < 32; m <<= 1)
+            for (int j = 0; j < RL; j++) {
+                f32x2 kk, qq;
+                lds(rows_at + j * RG * 16, kk, qq);
+                k01 = fma2(kk, S[j].x, k01);
+                k23 = fma2(kk, S[j].y, k23);
+                q01 = fma2(qq, S[j].x, q01);
+                q23 = fma2(qq, S[j].y, q23);
+            }
+            float ks[4], qs[4], vv[4], d[4], y[4];
+            split(k01, ks[0], ks[1]);
+            split(k23, ks[2], ks[3]);
+            split(q01, qs[0], qs[1]);
+            split(q23, qs[2], qs[3]);
+#pragma unroll
+            for (int m = CL; m < 32; m <<= 1)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    ks[e] += __shfl_xor_sync(0xffffffffu, ks[e], m);
+                    qs[e] += __shfl_xor_sync(0xffffffffu, qs[e], m);
+                }
+            const float4 gt = gates[t];
+            unpack4(vs[t][c0 / 4], vv);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                ks[e] += __shfl_xor_sync(0xffffffffu, ks[e], m);
-                qs[e] += __shfl_xor_sync(0xffffffffu, qs[e], m);
+                d[e] = gt.y * (vv[e] - gt.x * ks[e]);
+                y[e] = gt.x * qs[e] + gt.z * d[e];
             }
-        const float vv[4] = {__uint_as_float(vr.x << 16), __uint_as_float(vr.x & 0xffff0000u), __uint_as_float(vr.y << 16),
-                             __uint_as_float(vr.y & 0xffff0000u)};
-        float d[4], y[4];
+            if (r0 == 0) {
+                uint2 p;
+                p.x = pack2(y[0], y[1]);
+                p.y = pack2(y[2], y[3]);
+                *reinterpret_cast<uint2*>(o + (((size_t)sq.row0 + t0 + t) * H + h) * D + c0) = p;
+            }
+            const f32x2 decay = two(gt.x, gt.x), d01 = two(d[0], d[1]), d23 = two(d[2], d[3]);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            d[e] = b * (vv[e] - decay * ks[e]);
-            y[e] = decay * qs[e] + qk * d[e];
-        }
-        if (r0 == 0) {
-            uint2 p;
-            p.x = pack2(y[0], y[1]);
-            p.y = pack2(y[2], y[3]);
-            *reinterpret_cast<uint2*>(o + (row * H + h) * D + c0) = p;
-        }
-#pragma unroll
-        for (int j = 0; j < RL; j++) {
-            const float kc = kq[r0 + j * RG].x;
-            S[j].x = decay * S[j].x + kc * d[0];
-            S[j].y = decay * S[j].y + kc * d[1];
-            S[j].z = decay * S[j].z + kc * d[2];
-            S[j].w = decay * S[j].w + kc * d[3];
+            for (int j = 0; j < RL; j++) {
+                const f32x2 kk = lds_again(rows_at + j * RG * 16);
+                S[j].x = fma2(decay, S[j].x, mul2(kk, d01));
+                S[j].y = fma2(decay, S[j].y, mul2(kk, d23));
+            }
         }
     }
     if (sq.rows == 0 && sq.in == sq.out) return;
     float* dst = states + (size_t)sq.out * slot_stride + ((size_t)h * D + r0) * D + c0;
 #pragma unroll
-    for (int j = 0; j < RL; j++) *reinterpret_cast<float4*>(dst + (size_t)j * RG * D) = S[j];
+    for (int j = 0; j < RL; j++) *reinterpret_cast<ulonglong2*>(dst + (size_t)j * RG * D) = S[j];
 }
 
 // ---- convolution and gates ----
@@ -240,14 +295,13 @@ extern "C" int s1_gdn_step(const void* q, const void* k, const void* v, const fl
     if (!states || !aligned16(states)) return cudaErrorInvalidValue;
     if (rows > 0 && (!q || !k || !v || !g || !beta || !o || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)))
         return cudaErrorInvalidValue;
-    constexpr int CW = 32;
-    const long long units = (long long)nseq * H * (D / CW);
-    if (units > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const long long blocks = (long long)nseq * H;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     int* error = nullptr;
     const int rc = error_word(&error);
     if (rc != 0) return rc;
     const cudaError_t e =
-        launch_dep(gdn_step_kernel<CW>, (unsigned)((units + 3) / 4), 128, 0, as_stream(stream), static_cast<const bf16*>(q),
+        launch_dep(gdn_step_kernel, (unsigned)blocks, D / CW * 32, 0, as_stream(stream), static_cast<const bf16*>(q),
                    static_cast<const bf16*>(k), static_cast<const bf16*>(v), g, static_cast<const bf16*>(beta),
                    static_cast<bf16*>(o), H, H / HK, scale, states, slot_stride, seqs, error);
     return e != cudaSuccess ? e : cudaGetLastError();
