@@ -136,29 +136,33 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __g
 // Every key and value is read once for all query heads that share it (up to 16 of them, the rows of
 // an mma.m16n8k16), which gives at most 16 FLOP per byte: HBM bounds it, not the tensor pipe, and
 // tcgen05's 64-row minimum would idle three quarters and more of its rows. So: the copy engine streams
-// tiles of 64 tokens through a ring of shared memory that holds most of what an SM has, and four
-// warps work on them with plain warp-level MMAs.
+// tiles through a ring of shared memory that holds most of what an SM has, and four warps work on them
+// with plain warp-level MMAs.
 //
-// The work of a launch is one line of tiles (row by row, key-value head by key-value head, token
-// tiles of it) cut into equal runs, one per block, whatever the lengths are. A run's pieces that
-// cover a (row, head) whole are finished by the block; the others leave maximum, sum and weighted
-// values in float32 in the workspace, and a second kernel joins the parts of each in order.
-constexpr int TILE = 64;
+// A tile is HB neighbouring key-value heads (4, 2 or 1) of 16 * 4 / HB tokens: with 4 heads whole rows of
+// the pools, or whole kilobytes of them. A warp owns one head's 16 tokens of every tile, its running
+// maximum, sum and weighted values stay in its registers, and no warp waits for another until the
+// end of a piece, where warps of one head are summed.
+//
+// The work of a launch is one line of tiles (row by row, head block by head block, tokens in order)
+// cut into equal runs, one per block, whatever the lengths are. A run's pieces that cover a (row, head
+// block) whole are finished by the block; the others leave maximum, sum and weighted values in
+// float32 in the workspace, and a second kernel joins the parts of each in order.
 constexpr int CONSUMERS = 4, PAGED_THREADS = (CONSUMERS + 1) * 32;
+constexpr int SLICE = 16;       // tokens of a warp's part of a tile, and of a copied box
+constexpr int MIN_RUN = 2;      // tiles: a run of one saves nothing and leaves twice the parts to join
 constexpr int MAX_GROUP = 16;   // query heads of one key-value head that a block takes at once
 constexpr int MAX_BLOCKS = 296; // two per SM
 
 template <int DH>
 struct PCfg {
-    static constexpr int BLOCKS_PER_SM = 1;
-    static constexpr int HALF_BYTES = TILE * 128;                 // 64 dims of a tile
-    static constexpr int KV_BYTES = (DH / 64) * HALF_BYTES;
+    static constexpr int BLOCKS_PER_SM = DH == 128 ? 2 : 1;
+    static constexpr int STAGES = 3;
+    static constexpr int KV_BYTES = CONSUMERS * SLICE * DH * 2;
     static constexpr int STAGE = 2 * KV_BYTES;
-    static constexpr int STAGES = DH == 128 ? 6 : 3;
-    static constexpr int P_PITCH = TILE + 8;                      // bf16; 144 bytes, so that ldmatrix rows hit all banks
-    static constexpr int OFF_P = STAGES * STAGE;
-    static constexpr int OFF_F = OFF_P + 16 * P_PITCH * 2;        // float [4][16] maxima, [4][16] sums
-    static constexpr int OFF_BAR = OFF_F + 2 * CONSUMERS * 16 * 4;
+    static constexpr int OFF_SUM = STAGES * STAGE;                 // float [HB][16][64] for HB <= 2
+    static constexpr int OFF_ML = OFF_SUM + 2 * 16 * 64 * 4;       // float2 [4][16]
+    static constexpr int OFF_BAR = OFF_ML + CONSUMERS * 16 * 8;
     static constexpr int SMEM = OFF_BAR + 2 * STAGES * 8 + 64 + 1024;  // and what aligning the base takes
 };
 
@@ -169,7 +173,7 @@ struct PagedArgs {
     float* work;
     int* error;
     int rows, Hq, Hk, group, chunk, chunks;  // group = Hq / Hk in `chunks` parts of at most `chunk` heads
-    int box;                                 // token rows per copy: a power of two that divides a page
+    int units;                               // chunks * head blocks: what a row's tokens are walked for
     float scale_log2;
     PageTable table;
 };
@@ -177,31 +181,47 @@ struct PagedMaps {
     CUtensorMap k, v;
 };
 
-// Workspace: [blocks][2] parts of [chunk][DH] weighted values and [chunk] (maximum, sum) pairs, in whole
-// 16 bytes, then int4 [blocks] notes.
-__host__ __device__ inline size_t part_floats(int chunk, int DH) { return (size_t)chunk * DH + (2 * chunk + 3) / 4 * 4; }
+// Workspace: [blocks][2] parts of [heads][DH] weighted values and [heads] (maximum, sum) pairs, in whole
+// 16 bytes (heads = HB * chunk), then int4 [blocks] notes.
+__host__ __device__ inline size_t part_floats(int heads, int DH) { return (size_t)heads * DH + (2 * heads + 3) / 4 * 4; }
 
-// Tiles of a row over all its heads; 0 for a row that sits out, is empty or is refused.
+// Tiles of a row over all its units; 0 for a row that sits out, is empty or is refused.
+template <int TILE>
 __device__ __forceinline__ long long row_tiles(const PagedArgs& a, int r, int& tiles) {
     const int n = a.len[r], sq = a.seq ? a.seq[r] : r;
     tiles = 0;
     if (n <= 0 || sq < 0 || sq >= a.table.sequences || n > (long long)a.table.width * a.table.page_tokens) return 0;
     tiles = (n + TILE - 1) / TILE;
-    return (long long)tiles * a.Hk * a.chunks;
+    return (long long)tiles * a.units;
 }
+
+// The cut of a line of `total` tiles into runs, one per block, none of them empty but those behind the last.
+// (SMs do not stream equally fast: the first block ends some 15 % before the last. Equal runs over three
+// quarters and a finer cut of the rest, for the blocks that end first, was slower all the same, 103.7 -> 107 us
+// at 307,000 tokens of 4 heads: a block's start costs more than it evens out.)
+struct Cut {
+    long long total;
+    int runs;
+    Cut() = default;
+    __device__ Cut(long long t, int blocks) : total(t), runs((int)min((long long)blocks, (t + MIN_RUN - 1) / MIN_RUN)) {}
+    __device__ long long begin(int r) const { return r >= runs ? total : total * r / runs; }
+    // The last run that begins at or before tile t: floor(total r / runs) <= t just where r <= (runs (t + 1) - 1) / total.
+    __device__ int run_of(long long t) const { return (int)((runs * (t + 1) - 1) / total); }
+};
 
 // Position in the line of tiles.
 struct Walk {
-    int row, head, tile, tiles;  // head: key-value head * chunks + part of its group
+    int row, unit, tile, tiles;  // unit: head block * chunks + part of the groups
     long long left;
 };
+template <int TILE>
 __device__ __forceinline__ void walk_next_piece(const PagedArgs& a, Walk& w) {
     w.tile = 0;
-    if (++w.head < a.Hk * a.chunks) return;
-    w.head = 0;
+    if (++w.unit < a.units) return;
+    w.unit = 0;
     do {
         w.row++;
-    } while (w.row < a.rows && row_tiles(a, w.row, w.tiles) == 0);
+    } while (w.row < a.rows && row_tiles<TILE>(a, w.row, w.tiles) == 0);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -226,10 +246,12 @@ __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;
 
 __device__ __forceinline__ float gated(float o, float gate) { return o / (1.f + __expf(-gate)); }
 
-template <int DH>
+template <int DH, int HB>
 __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
     attn_paged_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ PagedMaps maps) {
     using G = PCfg<DH>;
+    constexpr int SUBS = CONSUMERS / HB, TILE = SLICE * SUBS;
+    constexpr int BOX_BYTES = HB * SLICE * DH * 2;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + G::OFF_BAR);
@@ -237,6 +259,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
     volatile int* gave_up = reinterpret_cast<volatile int*>(empty + G::STAGES);
     __shared__ long long warp_sums[PAGED_THREADS / 32];
     __shared__ Walk begin;
+    __shared__ Cut whole_cut;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     grid_dep_trigger();
@@ -259,7 +282,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
         long long mine = 0;
         for (int r = r0; r < r1; r++) {
             int tiles;
-            mine += row_tiles(a, r, tiles);
+            mine += row_tiles<TILE>(a, r, tiles);
         }
         long long upto = mine;
 #pragma unroll
@@ -275,19 +298,19 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
             if (w < warp) upto += warp_sums[w];
             total += warp_sums[w];
         }
-        // never an empty run between two others: the join follows a piece from block to block
-        const long long runs = min((long long)gridDim.x, total), b = blockIdx.x;
-        const long long lo = b < runs ? total * b / runs : total, hi = b < runs ? total * (b + 1) / runs : total;
+        const Cut cut(total, gridDim.x);
+        const long long lo = cut.begin(blockIdx.x), hi = cut.begin(blockIdx.x + 1);
+        if (tid == 0) whole_cut = cut;
         if (tid == 0 && lo == hi) begin.left = 0;
         if (lo < hi && upto - mine <= lo && lo < upto) {
             long long at = upto - mine;
             for (int r = r0; r < r1; r++) {
                 int tiles;
-                const long long n = row_tiles(a, r, tiles);
+                const long long n = row_tiles<TILE>(a, r, tiles);
                 if (lo < at + n) {
                     const int in_row = (int)(lo - at);  // below 2^31: the host limits a row's tiles
                     begin.row = r;
-                    begin.head = in_row / tiles;
+                    begin.unit = in_row / tiles;
                     begin.tile = in_row % tiles;
                     begin.tiles = tiles;
                     begin.left = hi - lo;
@@ -298,34 +321,23 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
         }
         __syncthreads();
     }
-    // rows without tiles: an empty one has nothing to attend to and gets zeros
-    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const int n = a.len[r], sq = a.seq ? a.seq[r] : r;
-        if (n < 0) continue;
-        if (sq < 0 || sq >= a.table.sequences || n > (long long)a.table.width * a.table.page_tokens) {
-            if (tid == 0) atomicCAS(a.error, 0, PAGED_BAD_ROW);
-        } else if (n == 0) {
-            uint32_t* z = reinterpret_cast<uint32_t*>(a.out + (size_t)r * a.Hq * DH);
-            for (int i = tid; i < a.Hq * DH / 2; i += PAGED_THREADS) z[i] = 0;
-        }
-    }
     Walk w = begin;
     auto fail = [&](int code) { atomicCAS(a.error, 0, code); };
 
     if (warp == CONSUMERS) {
-        // ---- copies: the whole warp walks, lane b looks up the page of box b, lane 0 issues ----
-        const int boxes = TILE / a.box;
+        // ---- copies: the whole warp walks, lane b looks up the page of box b and issues its copies ----
+        const uint64_t once = policy_evict_first();
         uint32_t it = 0;
         while (w.left > 0) {
             const int n = a.len[w.row], sq = a.seq ? a.seq[w.row] : w.row;
             const int* pages = a.table.pages + (size_t)sq * a.table.width;
-            const int hk = w.head / a.chunks;
+            const int column = w.unit / a.chunks * (HB * DH / 64);
             const int end = (int)min((long long)w.tiles, w.tile + w.left);
             for (; w.tile < end; w.tile++, w.left--, it++) {
                 const int stage = it % G::STAGES;
-                const int t = w.tile * TILE + lane * a.box;
+                const int t = w.tile * TILE + lane * SLICE;
                 int at = -1;  // the box's first row in the pools
-                if (lane < boxes && t < n) {
+                if (lane < SUBS && t < n) {
                     const int slot = t / a.table.page_tokens;
                     int page = pages[slot];
                     if (page < 0 || page >= a.table.n_pages) {
@@ -341,34 +353,32 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                     break;
                 }
                 const int have = __popc(__ballot_sync(0xffffffffu, at >= 0));
-                if (lane == 0) mbar_expect_tx(&full[stage], (uint32_t)have * a.box * DH * 4);
+                if (lane == 0) mbar_expect_tx(&full[stage], (uint32_t)have * 2 * BOX_BYTES);
                 __syncwarp();
                 if (at >= 0) {
-                    unsigned char* dst = smem + stage * G::STAGE + lane * a.box * 128;
-#pragma unroll
-                    for (int c = 0; c < DH / 64; c++) {
-                        tma_load_2d(dst + c * G::HALF_BYTES, &maps.k, hk * DH + c * 64, at, &full[stage]);
-                        tma_load_2d(dst + G::KV_BYTES + c * G::HALF_BYTES, &maps.v, hk * DH + c * 64, at, &full[stage]);
-                    }
+                    unsigned char* dst = smem + stage * G::STAGE + lane * BOX_BYTES;
+                    tma_load_3d(dst, &maps.k, 0, at, column, &full[stage], once);
+                    tma_load_3d(dst + G::KV_BYTES, &maps.v, 0, at, column, &full[stage], once);
                 }
             }
-            if (w.left > 0) walk_next_piece(a, w);
+            if (w.left > 0) walk_next_piece<TILE>(a, w);
         }
     } else {
-        constexpr int DW = DH / CONSUMERS, NT = DW / 8;  // dims of the result per warp, in n-tiles of 8
-        const uint32_t p_addr = smem_addr(smem + G::OFF_P);
-        float* wmax = reinterpret_cast<float*>(smem + G::OFF_F);
-        float* wsum = wmax + CONSUMERS * 16;
-        const int ra = lane >> 2, rb = ra + 8;  // the two rows (query heads) of this lane's accumulators
-        // lane parts of the ldmatrix addresses
-        const int k_tok = warp * 16 + (lane >> 4) * 8 + (lane & 7), k_ch = (lane >> 3) & 1;
-        const int v_tok = ((lane >> 3) & 1) * 8 + (lane & 7), v_ch = warp * (DW / 8) + (lane >> 4);
-        int4 note = make_int4(-1, 0, 0, 0);
+        constexpr int NT = DH / 8;                          // n-tiles of 8 dims of the result
+        const int mine = warp % HB, sub = warp / HB;        // this warp's head of the block, its slice of the tile
+        float* sums = reinterpret_cast<float*>(smem + G::OFF_SUM);
+        float2* ml = reinterpret_cast<float2*>(smem + G::OFF_ML);
+        const int ra = lane >> 2, rb = ra + 8;              // the two rows (query heads) of this lane's accumulators
+        // lane parts of the ldmatrix addresses in the box's tile of 64 dims
+        const int k_tok = (lane >> 4) * 8 + (lane & 7), k_ch = (lane >> 3) & 1;
+        const int v_tok = lane & 15, v_ch = lane >> 4;
+        const uint32_t my_tiles = sub * BOX_BYTES + mine * (DH / 64) * (SLICE * 128);
+        int4 note = make_int4(-1, 0, 0, 0);  // row and unit that begin here and go on, the block of their last part
         uint32_t it = 0;
         bool ok = true;
         while (w.left > 0) {
             const int n = a.len[w.row];
-            const int hk = w.head / a.chunks, part = w.head % a.chunks;
+            const int hk = w.unit / a.chunks * HB + mine, part = w.unit % a.chunks;
             const int h0 = part * a.chunk, heads = min(a.chunk, a.group - h0);
             const size_t q_row = ((size_t)w.row * a.Hq + (size_t)hk * a.group + h0) * DH;
             uint32_t qf[DH / 16][4];
@@ -392,77 +402,69 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                     *gave_up = 1;
                     ok = false;
                 }
-                const uint32_t kb = smem_addr(smem + stage * G::STAGE), vb = kb + G::KV_BYTES;
-                float s[2][4] = {};
+                const int left = n - w.tile * TILE - sub * SLICE;  // valid tokens of the slice, from its first on
+                if (left > 0) {
+                    const uint32_t kb = smem_addr(smem + stage * G::STAGE) + my_tiles, vb = kb + G::KV_BYTES;
+                    float s[2][4] = {}, s2[2][4] = {};  // two chains each, so that the products wait less for one another
 #pragma unroll
-                for (int ks = 0; ks < DH / 16; ks++) {
-                    const int ch = ks * 2 + k_ch;
-                    uint32_t b[4];
-                    ldsm4(b, kb + (ch >> 3) * G::HALF_BYTES + k_tok * 128 + (((ch ^ k_tok) & 7) << 4));
-                    mma16816(s[0], qf[ks], b[0], b[1]);
-                    mma16816(s[1], qf[ks], b[2], b[3]);
-                }
-                const int left = n - w.tile * TILE;  // valid tokens of the tile, from its first on
-                const int c0 = warp * 16 + (lane & 3) * 2;
-                float xa = -INFINITY, xb = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const bool in = c0 + j * 8 + e < left;
-                        s[j][e] = in ? s[j][e] * a.scale_log2 : -INFINITY;
-                        s[j][2 + e] = in ? s[j][2 + e] * a.scale_log2 : -INFINITY;
-                        xa = fmaxf(xa, s[j][e]);
-                        xb = fmaxf(xb, s[j][2 + e]);
+                    for (int ks = 0; ks < DH / 16; ks++) {
+                        const int ch = ks * 2 + k_ch;
+                        uint32_t b[4];
+                        ldsm4(b, kb + (ch >> 3) * (SLICE * 128) + k_tok * 128 + (((ch ^ k_tok) & 7) << 4));
+                        mma16816(ks & 1 ? s2[0] : s[0], qf[ks], b[0], b[1]);
+                        mma16816(ks & 1 ? s2[1] : s[1], qf[ks], b[2], b[3]);
                     }
+                    float xa = -INFINITY, xb = -INFINITY;
 #pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, o));
-                    xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, o));
-                }
-                if ((lane & 3) == 0) wmax[warp * 16 + ra] = xa, wmax[warp * 16 + rb] = xb;
-                consumer_sync();
-                float na = ma, nb = mb;
+                    for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int i = 0; i < CONSUMERS; i++) na = fmaxf(na, wmax[i * 16 + ra]), nb = fmaxf(nb, wmax[i * 16 + rb]);
-                // a row without a finite score so far keeps offset 0: its terms are exp2(-inf) = 0
-                const float oa = na == -INFINITY ? 0.f : na, ob = nb == -INFINITY ? 0.f : nb;
-                const float fa = exp2f(ma - oa), fb = exp2f(mb - ob);
-                ma = na, mb = nb;
-                la *= fa, lb *= fb;
+                        for (int e = 0; e < 2; e++) {
+                            const bool in = j * 8 + (lane & 3) * 2 + e < left;
+                            s[j][e] = in ? (s[j][e] + s2[j][e]) * a.scale_log2 : -INFINITY;
+                            s[j][2 + e] = in ? (s[j][2 + e] + s2[j][2 + e]) * a.scale_log2 : -INFINITY;
+                            xa = fmaxf(xa, s[j][e]);
+                            xb = fmaxf(xb, s[j][2 + e]);
+                        }
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float p0 = exp2f(s[j][0] - oa), p1 = exp2f(s[j][1] - oa), p2 = exp2f(s[j][2] - ob), p3 = exp2f(s[j][3] - ob);
-                    la += p0 + p1, lb += p2 + p3;
-                    const uint32_t at = p_addr + (uint32_t)(c0 + j * 8) * 2;
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + ra * G::P_PITCH * 2), "r"(pack2(p0, p1)) : "memory");
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + rb * G::P_PITCH * 2), "r"(pack2(p2, p3)) : "memory");
-                }
+                    for (int o = 1; o < 4; o <<= 1) {
+                        xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, o));
+                        xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, o));
+                    }
+                    if (__any_sync(0xffffffffu, xa > ma || xb > mb)) {
+                        const float na = fmaxf(ma, xa), nb = fmaxf(mb, xb);
+                        const float fa = ma == -INFINITY ? 0.f : exp2f(ma - na), fb = mb == -INFINITY ? 0.f : exp2f(mb - nb);
+                        ma = na, mb = nb;
+                        la *= fa, lb *= fb;
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[t][0] *= fa, acc[t][1] *= fa, acc[t][2] *= fb, acc[t][3] *= fb;
-                consumer_sync();
-#pragma unroll
-                for (int ks = 0; ks < TILE / 16; ks++) {
+                        for (int t = 0; t < NT; t++) acc[t][0] *= fa, acc[t][1] *= fa, acc[t][2] *= fb, acc[t][3] *= fb;
+                    }
+                    // a row without a finite score so far keeps offset 0: its terms are exp2(-inf) = 0
+                    const float oa = ma == -INFINITY ? 0.f : ma, ob = mb == -INFINITY ? 0.f : mb;
                     uint32_t pf[4];
-                    ldsm4(pf, p_addr + ((lane & 15) * G::P_PITCH + ks * 16 + (lane >> 4) * 8) * 2);
-                    const int tok = ks * 16 + v_tok;
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const float p0 = exp2f(s[j][0] - oa), p1 = exp2f(s[j][1] - oa), p2 = exp2f(s[j][2] - ob), p3 = exp2f(s[j][3] - ob);
+                        la += p0 + p1, lb += p2 + p3;
+                        pf[2 * j] = pack2(p0, p1);
+                        pf[2 * j + 1] = pack2(p2, p3);
+                    }
                     // values behind the last token may be anything, NaN included: their products with a
                     // probability of zero have to be zero
-                    const bool tail = ks * 16 + 16 > left;
+                    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+                    if (left < SLICE) {
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int t0 = e * 8 + (lane & 3) * 2;
+                            keep[e] = (t0 < left ? 0xffffu : 0u) | (t0 + 1 < left ? 0xffff0000u : 0u);
+                        }
+                    }
 #pragma unroll
                     for (int t = 0; t < NT; t += 2) {
                         const int ch = v_ch + t;
                         uint32_t b[4];
-                        ldsm4_t(b, vb + (ch >> 3) * G::HALF_BYTES + tok * 128 + (((ch ^ tok) & 7) << 4));
-                        if (tail) {
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int t0 = ks * 16 + (e & 1) * 8 + (lane & 3) * 2;
-                                b[e] &= (t0 < left ? 0xffffu : 0u) | (t0 + 1 < left ? 0xffff0000u : 0u);
-                            }
-                        }
-                        mma16816(acc[t], pf, b[0], b[1]);
-                        mma16816(acc[t + 1], pf, b[2], b[3]);
+                        ldsm4_t(b, vb + (ch >> 3) * (SLICE * 128) + v_tok * 128 + (((ch ^ v_tok) & 7) << 4));
+                        mma16816(acc[t], pf, b[0] & keep[0], b[1] & keep[1]);
+                        mma16816(acc[t + 1], pf, b[2] & keep[0], b[3] & keep[1]);
                     }
                 }
                 __syncwarp();
@@ -475,17 +477,51 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                 la += __shfl_xor_sync(0xffffffffu, la, o);
                 lb += __shfl_xor_sync(0xffffffffu, lb, o);
             }
-            if ((lane & 3) == 0) wsum[warp * 16 + ra] = la, wsum[warp * 16 + rb] = lb;
-            consumer_sync();
-            la = lb = 0.f;
+            if constexpr (SUBS > 1) {
+                // one maximum for the warps of a head, then their sums and weighted values in turn
+                if ((lane & 3) == 0) ml[warp * 16 + ra] = make_float2(ma, la), ml[warp * 16 + rb] = make_float2(mb, lb);
+                consumer_sync();
+                float na = -INFINITY, nb = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < CONSUMERS; i++) la += wsum[i * 16 + ra], lb += wsum[i * 16 + rb];
+                for (int u = 0; u < SUBS; u++) na = fmaxf(na, ml[(u * HB + mine) * 16 + ra].x), nb = fmaxf(nb, ml[(u * HB + mine) * 16 + rb].x);
+                const float oa = na == -INFINITY ? 0.f : na, ob = nb == -INFINITY ? 0.f : nb;
+                const float fa = exp2f(ma - oa), fb = exp2f(mb - ob);
+                la = lb = 0.f;
+#pragma unroll
+                for (int u = 0; u < SUBS; u++) {
+                    const float2 x = ml[(u * HB + mine) * 16 + ra], y = ml[(u * HB + mine) * 16 + rb];
+                    la += x.y * exp2f(x.x - oa), lb += y.y * exp2f(y.x - ob);
+                }
+                ma = na, mb = nb;
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[t][0] *= fa, acc[t][1] *= fa, acc[t][2] *= fb, acc[t][3] *= fb;
+#pragma unroll
+                for (int u = 1; u < SUBS; u++)
+#pragma unroll
+                    for (int c = 0; c < NT; c += 8) {
+                        float2* box = reinterpret_cast<float2*>(sums + mine * 16 * 64);
+#pragma unroll
+                        for (int t = 0; t < 8; t++)
+                            if (sub == u) {
+                                box[(t * 2) * 32 + lane] = make_float2(acc[c + t][0], acc[c + t][1]);
+                                box[(t * 2 + 1) * 32 + lane] = make_float2(acc[c + t][2], acc[c + t][3]);
+                            }
+                        consumer_sync();
+#pragma unroll
+                        for (int t = 0; t < 8; t++)
+                            if (sub == 0) {
+                                const float2 x = box[(t * 2) * 32 + lane], y = box[(t * 2 + 1) * 32 + lane];
+                                acc[c + t][0] += x.x, acc[c + t][1] += x.y, acc[c + t][2] += y.x, acc[c + t][3] += y.y;
+                            }
+                        consumer_sync();
+                    }
+            }
             const bool whole = from == 0 && end == w.tiles;
-            if (whole) {
+            if (sub == 0 && whole) {
                 const float ia = la == 0.f ? 0.f : 1.f / la, ib = lb == 0.f ? 0.f : 1.f / lb;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const size_t at = q_row + warp * DW + t * 8 + (lane & 3) * 2;
+                    const size_t at = q_row + t * 8 + (lane & 3) * 2;
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int row = e ? rb : ra;
@@ -499,95 +535,168 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                         *reinterpret_cast<uint32_t*>(a.out + at + (size_t)row * DH) = pack2(y0, y1);
                     }
                 }
-            } else {
-                // the part that begins a (row, head) lies in place 1, one that continues it in place 0
+            } else if (sub == 0) {
+                // the part that begins a (row, unit) lies in place 1, one that continues it in place 0
                 const int place = from == 0 ? 1 : 0;
-                float* dst = a.work + ((size_t)blockIdx.x * 2 + place) * part_floats(a.chunk, DH);
+                float* dst = a.work + ((size_t)blockIdx.x * 2 + place) * part_floats(HB * a.chunk, DH);
+                float* val = dst + (size_t)mine * a.chunk * DH;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const int d = warp * DW + t * 8 + (lane & 3) * 2;
-                    if (ra < heads) *reinterpret_cast<float2*>(dst + ra * DH + d) = make_float2(acc[t][0], acc[t][1]);
-                    if (rb < heads) *reinterpret_cast<float2*>(dst + rb * DH + d) = make_float2(acc[t][2], acc[t][3]);
+                    const int d = t * 8 + (lane & 3) * 2;
+                    if (ra < heads) *reinterpret_cast<float2*>(val + ra * DH + d) = make_float2(acc[t][0], acc[t][1]);
+                    if (rb < heads) *reinterpret_cast<float2*>(val + rb * DH + d) = make_float2(acc[t][2], acc[t][3]);
                 }
-                float* ml = dst + a.chunk * DH;
-                if (warp == 0 && (lane & 3) == 0) {
-                    if (ra < heads) ml[2 * ra] = ma, ml[2 * ra + 1] = la;
-                    if (rb < heads) ml[2 * rb] = mb, ml[2 * rb + 1] = lb;
+                float2* pair = reinterpret_cast<float2*>(dst + (size_t)HB * a.chunk * DH) + mine * a.chunk;
+                if ((lane & 3) == 0) {
+                    if (ra < heads) pair[ra] = make_float2(ma, la);
+                    if (rb < heads) pair[rb] = make_float2(mb, lb);
                 }
-                if (place == 1)
-                    note.x = w.row, note.y = w.head;
-                else
-                    note.z = end == w.tiles ? 2 : 1;
             }
-            if (w.left > 0) walk_next_piece(a, w);
+            if (from == 0 && !whole) {
+                // it ends this run, and its last tile lies that far behind the run's end
+                const Cut cut = whole_cut;
+                note = make_int4(w.row, w.unit, cut.run_of(cut.begin(blockIdx.x + 1) + w.tiles - end - 1), 0);
+            }
+            if (w.left > 0) walk_next_piece<TILE>(a, w);
         }
         if (tid == 0)
-            reinterpret_cast<int4*>(a.work + (size_t)gridDim.x * 2 * part_floats(a.chunk, DH))[blockIdx.x] = note;
+            reinterpret_cast<int4*>(a.work + (size_t)gridDim.x * 2 * part_floats(HB * a.chunk, DH))[blockIdx.x] = note;
+    }
+    // rows without tiles: an empty one has nothing to attend to and gets zeros
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const int n = a.len[r], sq = a.seq ? a.seq[r] : r;
+        if (n < 0) continue;
+        if (sq < 0 || sq >= a.table.sequences || n > (long long)a.table.width * a.table.page_tokens) {
+            if (tid == 0) atomicCAS(a.error, 0, PAGED_BAD_ROW);
+        } else if (n == 0) {
+            uint32_t* z = reinterpret_cast<uint32_t*>(a.out + (size_t)r * a.Hq * DH);
+            for (int i = tid; i < a.Hq * DH / 2; i += PAGED_THREADS) z[i] = 0;
+        }
     }
     // after an abort give copies in flight time to land before the shared memory is released
     if (*gave_up) __nanosleep(1000000);
     __syncthreads();
 }
 
-// Joins the parts of the (row, head)s that were cut: block (b, i) takes query head i of the one that
-// begins in block b of the first kernel and goes on in the blocks after it, if there is one. The
-// order of the sums is fixed by the cut alone.
-constexpr int JOIN_WARPS = 8;
+// Joins the parts of the (row, unit)s that were cut. One begins in some block of the first kernel (its
+// place 1) and goes on in the blocks after it (their place 0); that block's note says up to which. The
+// items are the query heads of these; a warp takes one at a time, or a whole block where items are
+// few. The order of the sums is fixed by the cut alone. All of this is a chain of a few trips to L2 behind the
+// first kernel's end, so the code is kept short: unrolled further it took longer to fetch than to run.
+constexpr int JOIN_WARPS = 16, JOIN_BLOCKS = 148;
+
 template <int DH>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) attn_paged_join_kernel(const __grid_constant__ PagedArgs a, int blocks) {
-    constexpr int E = DH / 32;
-    __shared__ float sums[JOIN_WARPS][DH];
-    __shared__ int stop;
+__global__ void __launch_bounds__(JOIN_WARPS * 32) attn_paged_join_kernel(const __grid_constant__ PagedArgs a, int blocks, int HB) {
+    constexpr int E = DH / 128, U = 6;  // parts in flight per warp
+    __shared__ int4 notes[MAX_BLOCKS];
+    __shared__ int begins[MAX_BLOCKS], base[JOIN_WARPS];
+    __shared__ __align__(16) float sums[JOIN_WARPS][DH];
+    __shared__ float2 pairs[JOIN_WARPS];
     grid_dep_trigger();
     grid_dep_sync();
-    const int b = blockIdx.x, i = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const size_t floats = part_floats(a.chunk, DH);
-    const int4* notes = reinterpret_cast<const int4*>(a.work + (size_t)blocks * 2 * floats);
-    const int4 mine = notes[b];
-    if (mine.x < 0) return;
-    const int hk = mine.y / a.chunks, h0 = mine.y % a.chunks * a.chunk;
-    if (i >= min(a.chunk, a.group - h0)) return;
-    if (threadIdx.x == 0) stop = blocks;
-    __syncthreads();
-    for (int j = b + 1 + threadIdx.x; j < blocks; j += JOIN_WARPS * 32)
-        if (notes[j].z != 1) atomicMin(&stop, j);
-    __syncthreads();
-    const int parts = min(stop, blocks - 1) - b + 1;  // b's place 1, then place 0 of b + 1 .. stop
-    auto part = [&](int p) { return a.work + ((size_t)(b + p) * 2 + (p == 0)) * floats; };
-    float m = -INFINITY;
-    for (int p = lane; p < parts; p += 32) m = fmaxf(m, part(p)[a.chunk * DH + 2 * i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (m == -INFINITY) m = 0.f;
-    float l = 0.f;
-    for (int p = lane; p < parts; p += 32) {
-        const float* ml = part(p) + a.chunk * DH + 2 * i;
-        l += ml[1] * exp2f(ml[0] - m);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int heads = HB * a.chunk;
+    const size_t floats = part_floats(heads, DH);
+    const int4* src = reinterpret_cast<const int4*>(a.work + (size_t)blocks * 2 * floats);
+    // the blocks in which one begins, in a list
+    int count = 0;
+    for (int j0 = 0; j0 < blocks; j0 += JOIN_WARPS * 32) {
+        const int j = j0 + tid;
+        const int4 note = j < blocks ? src[j] : make_int4(-1, 0, 0, 0);
+        const uint32_t all = __ballot_sync(0xffffffffu, note.x >= 0);
+        if (lane == 0) base[warp] = __popc(all);
+        __syncthreads();
+        int at = count;
+        for (int w = 0; w < JOIN_WARPS; w++) {
+            if (w < warp) at += base[w];
+            count += base[w];
+        }
+        if (note.x >= 0) {
+            notes[j] = note;
+            begins[at + __popc(all & ((1u << lane) - 1))] = j;
+        }
+        __syncthreads();
     }
-    l = warp_sum(l);
-    float acc[E] = {};
-    for (int p = warp; p < parts; p += JOIN_WARPS) {
-        const float* src = part(p);
-        const float f = exp2f(src[a.chunk * DH + 2 * i] - m);
+    const int items = count * heads;
+    const bool together = items <= 2 * (int)gridDim.x;
+    const int width = together ? 1 : JOIN_WARPS;
+    for (int item = blockIdx.x * width + (together ? 0 : warp); item < items; item += gridDim.x * width) {
+        const int b = begins[item / heads], slot = item % heads, of = slot / a.chunk, i = slot % a.chunk;
+        const int4 note = notes[b];
+        const int hk = note.y / a.chunks * HB + of, h0 = note.y % a.chunks * a.chunk;
+        if (i >= min(a.chunk, a.group - h0)) continue;
+        const size_t at = ((size_t)note.x * a.Hq + (size_t)hk * a.group + h0 + i) * DH;
+        float m = -INFINITY, l = 0.f;
+        float4 acc[E] = {};
+        const int stride = together ? JOIN_WARPS : 1;
+        for (int p0 = b + (together ? warp : 0); p0 <= note.z; p0 += U * stride) {
+            float2 ml[U];
+            float4 x[U][E];
 #pragma unroll
-        for (int e = 0; e < E; e += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(src + (size_t)i * DH + e * 32 + lane * 4);
-            acc[e] += f * x.x, acc[e + 1] += f * x.y, acc[e + 2] += f * x.z, acc[e + 3] += f * x.w;
+            for (int u = 0; u < U; u++) {
+                const int p = p0 + u * stride;
+                ml[u] = make_float2(-INFINITY, 0.f);
+                if (p <= note.z) {
+                    const float* part = a.work + ((size_t)p * 2 + (p == b)) * floats;
+                    ml[u] = reinterpret_cast<const float2*>(part + (size_t)heads * DH)[slot];
+#pragma unroll
+                    for (int e = 0; e < E; e++) x[u][e] = *reinterpret_cast<const float4*>(part + (size_t)slot * DH + e * 128 + lane * 4);
+                }
+            }
+            float mm = m;
+#pragma unroll
+            for (int u = 0; u < U; u++) mm = fmaxf(mm, ml[u].x);
+            const float off = mm == -INFINITY ? 0.f : mm, f = exp2f(m - off);
+            m = mm, l *= f;
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[e].x *= f, acc[e].y *= f, acc[e].z *= f, acc[e].w *= f;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (p0 + u * stride <= note.z) {
+                    const float c = exp2f(ml[u].x - off);
+                    l += ml[u].y * c;
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        acc[e].x += c * x[u][e].x, acc[e].y += c * x[u][e].y, acc[e].z += c * x[u][e].z, acc[e].w += c * x[u][e].w;
+                }
+        }
+        if (together) {
+#pragma unroll
+            for (int e = 0; e < E; e++) *reinterpret_cast<float4*>(&sums[warp][e * 128 + lane * 4]) = acc[e];
+            if (lane == 0) pairs[warp] = make_float2(m, l);
+            __syncthreads();
+            m = -INFINITY;
+            for (int w = 0; w < JOIN_WARPS; w++) m = fmaxf(m, pairs[w].x);
+            const float off = m == -INFINITY ? 0.f : m;
+            l = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (warp == 0)
+                for (int w = 0; w < JOIN_WARPS; w++) {
+                    const float c = exp2f(pairs[w].x - off);
+                    l += pairs[w].y * c;
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const float4 x = *reinterpret_cast<const float4*>(&sums[w][e * 128 + lane * 4]);
+                        acc[e].x += c * x.x, acc[e].y += c * x.y, acc[e].z += c * x.z, acc[e].w += c * x.w;
+                    }
+                }
+            __syncthreads();
+        }
+        if (together && warp > 0) continue;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const size_t d = at + e * 128 + lane * 4;
+            float y[4] = {acc[e].x * inv, acc[e].y * inv, acc[e].z * inv, acc[e].w * inv};
+            if (a.gate) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) y[k] = gated(y[k], f32(a.gate[d + k]));
+            }
+            *reinterpret_cast<uint32_t*>(a.out + d) = pack2(y[0], y[1]);
+            *reinterpret_cast<uint32_t*>(a.out + d + 2) = pack2(y[2], y[3]);
         }
     }
-#pragma unroll
-    for (int e = 0; e < E; e += 4)
-        *reinterpret_cast<float4*>(&sums[warp][e * 32 + lane * 4]) = make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= DH) return;
-    float y = 0.f;
-#pragma unroll
-    for (int w = 0; w < JOIN_WARPS; w++) y += sums[w][d];
-    y = l == 0.f ? 0.f : y / l;
-    const size_t at = ((size_t)mine.x * a.Hq + (size_t)hk * a.group + h0 + i) * DH + d;
-    if (a.gate) y = gated(y, f32(a.gate[at]));
-    a.out[at] = to_bf16(y);
 }
 
 // The attention family's error word on the current device, looked up once per device.
@@ -611,20 +720,31 @@ bool table_ok(const PageTable& t) {
            (long long)t.n_pages * t.page_tokens <= 0x7fffffffLL && (long long)t.width * t.page_tokens <= (1LL << 30);
 }
 
-template <int DH>
+// Key-value heads of a tile: as many as share the pool's rows, up to a warp each.
+inline int head_block(int Hk) { return Hk % 4 == 0 ? 4 : Hk % 2 == 0 ? 2 : 1; }
+
+template <int DH, int HB>
 int run_paged(const PagedArgs& a, const PagedMaps& maps, int dev, int blocks, cudaStream_t st) {
     using G = PCfg<DH>;
     static bool configured[64] = {};
     if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_paged_kernel<DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(attn_paged_kernel<DH, HB>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
         if (e != cudaSuccess) return e;
         configured[dev] = true;
     }
-    cudaError_t e = launch_dep_family(DEP_ATTENTION, attn_paged_kernel<DH>, blocks, PAGED_THREADS, G::SMEM, st, a, maps);
+    cudaError_t e = launch_dep_family(DEP_ATTENTION, attn_paged_kernel<DH, HB>, blocks, PAGED_THREADS, G::SMEM, st, a, maps);
     if (e != cudaSuccess) return e;
     // always a programmatic dependent: it waits for the first kernel before it reads anything
-    e = launch_maybe_dep(true, attn_paged_join_kernel<DH>, dim3(blocks, a.chunk), JOIN_WARPS * 32, 0, st, a, blocks);
+    e = launch_maybe_dep(true, attn_paged_join_kernel<DH>, JOIN_BLOCKS, JOIN_WARPS * 32, 0, st, a, blocks,
+                         HB);
     return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int DH>
+int run_paged(int HB, const PagedArgs& a, const PagedMaps& maps, int dev, int blocks, cudaStream_t st) {
+    return HB == 4   ? run_paged<DH, 4>(a, maps, dev, blocks, st)
+           : HB == 2 ? run_paged<DH, 2>(a, maps, dev, blocks, st)
+                     : run_paged<DH, 1>(a, maps, dev, blocks, st);
 }
 
 }  // namespace
@@ -668,7 +788,8 @@ extern "C" int s1_attn_prep_paged(const void* qg, const void* kr, const void* vr
 
 extern "C" size_t s1_attention_paged_workspace_floats(int Hq, int Hk, int Dh) {
     if (Hq <= 0 || Hk <= 0 || Hq % Hk != 0 || (Dh != 128 && Dh != 256)) return 0;
-    return (size_t)MAX_BLOCKS * (2 * part_floats(std::min(Hq / Hk, MAX_GROUP), Dh) + 4);
+    const int group = Hq / Hk, chunks = (group + MAX_GROUP - 1) / MAX_GROUP;
+    return (size_t)MAX_BLOCKS * (2 * part_floats(head_block(Hk) * ((group + chunks - 1) / chunks), Dh) + 4);
 }
 
 extern "C" int s1_attention_paged(const void* q, const void* gate, void* out, const void* k_pages, const void* v_pages,
@@ -689,12 +810,14 @@ extern "C" int s1_attention_paged(const void* q, const void* gate, void* out, co
     a.group = Hq / Hk;
     a.chunks = (a.group + MAX_GROUP - 1) / MAX_GROUP;
     a.chunk = (a.group + a.chunks - 1) / a.chunks;
-    const long long row_most = ((long long)table_pages * page_tokens + TILE - 1) / TILE * Hk * a.chunks;
+    const int HB = head_block(Hk), tile = SLICE * CONSUMERS / HB;
+    if ((long long)(Hk / HB) * a.chunks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    a.units = Hk / HB * a.chunks;
+    const long long row_most = ((long long)table_pages * page_tokens + tile - 1) / tile * a.units;
     if (row_most > 0x7fffffffLL) return cudaErrorInvalidValue;
     a.q = static_cast<const bf16*>(q), a.gate = static_cast<const bf16*>(gate), a.out = static_cast<bf16*>(out);
     a.seq = seq, a.len = len, a.work = workspace, a.rows = rows, a.Hq = Hq, a.Hk = Hk, a.table = t;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.box = page_tokens % 64 == 0 ? 64 : page_tokens % 32 == 0 ? 32 : 16;
     int dev = 0;
     const int rc = error_word(&a.error, &dev);
     if (rc != 0) return rc;
@@ -705,10 +828,10 @@ extern "C" int s1_attention_paged(const void* q, const void* gate, void* out, co
     }
     PagedMaps maps;
     const uint64_t pool_rows = (uint64_t)n_pages * page_tokens, width = (uint64_t)Hk * Dh;
-    if (!tensor_map_2d(k_pages, pool_rows, width, width, a.box, &maps.k) ||
-        !tensor_map_2d(v_pages, pool_rows, width, width, a.box, &maps.v))
+    if (!tensor_map_columns(k_pages, pool_rows, width, SLICE, HB * Dh, &maps.k) ||
+        !tensor_map_columns(v_pages, pool_rows, width, SLICE, HB * Dh, &maps.v))
         return CS1_ERR_TENSOR_MAP;
     const int per_sm = Dh == 256 ? PCfg<256>::BLOCKS_PER_SM : PCfg<128>::BLOCKS_PER_SM;
     const int blocks = (int)std::min<long long>(std::min(MAX_BLOCKS, sm_count[dev] * per_sm), rows * row_most);
-    return Dh == 256 ? run_paged<256>(a, maps, dev, blocks, as_stream(stream)) : run_paged<128>(a, maps, dev, blocks, as_stream(stream));
+    return Dh == 256 ? run_paged<256>(HB, a, maps, dev, blocks, as_stream(stream)) : run_paged<128>(HB, a, maps, dev, blocks, as_stream(stream));
 }

@@ -76,6 +76,18 @@ bool encode(const void* ptr, uint64_t rows, uint64_t cols, uint64_t row_stride, 
 
 }  // namespace
 
+bool tensor_map_columns(const void* ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols, CUtensorMap* out) {
+    EncodeTiled fn = encode_fn();
+    if (!fn || rows == 0 || cols == 0 || cols % 64 != 0 || box_cols % 64 != 0 || box_cols == 0) return false;
+    const cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)cols / 64};
+    const cuuint64_t strides[2] = {(cuuint64_t)cols * 2, 128};
+    const cuuint32_t box[3] = {64, box_rows, box_cols / 64};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool tensor_map_2d(const void* ptr, uint64_t rows, uint64_t cols, uint64_t row_stride, uint32_t box_rows,
                    CUtensorMap* out) {
     return encode(ptr, rows, cols, row_stride, box_rows, 0, out);

@@ -14,4 +14,8 @@ bool tensor_map_2d(const void* ptr, uint64_t rows, uint64_t cols, uint64_t row_s
 // most 256 columns) land densely packed, row after row.
 bool tensor_map_2d_plain(const void* ptr, uint64_t rows, uint64_t cols, uint64_t row_stride, uint32_t box_rows,
                          uint32_t box_cols, CUtensorMap* out);
+// Tensor map of a dense row-major bf16 matrix [rows, cols] as [cols / 64][rows][64], read in boxes of
+// box_rows rows by box_cols columns (multiples of 64): a box lands as one [box_rows, 64] tile with the
+// 128-byte swizzle per 64 columns, one tile after the other. Not cached.
+bool tensor_map_columns(const void* ptr, uint64_t rows, uint64_t cols, uint32_t box_rows, uint32_t box_cols, CUtensorMap* out);
 }  // namespace s1
