@@ -3,6 +3,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -54,6 +55,7 @@ def build(verbose=False, force=False, ptxas_info=False):
         cmd = [NVCC, "-shared", "-o", OUT] + objs + ["-L" + lib64, "-ldl", "-Xlinker", "-rpath", "-Xlinker", lib64]
         subprocess.run(cmd, check=True)
     build_compare()
+    build_fastcall()
     return OUT
 
 
@@ -65,6 +67,16 @@ def build_compare():
         lib64 = os.path.join(CUDA_HOME, "lib64")
         subprocess.run([NVCC, "-O2", "-std=c++17", "-shared", "-Xcompiler", "-fPIC", "-o", out, src, "-L" + lib64,
                         "-lcublasLt", "-Xlinker", "-rpath", "-Xlinker", lib64], check=True)
+    return out
+
+
+def build_fastcall():
+    """The direct binding of the step operators (a CPython extension; lib.py uses ctypes where it is absent)."""
+    src = os.path.join(PKG, "binding", "fastcall.cpp")
+    out = os.path.join(PKG, "_fastcall.so")
+    if _stale(out, [src, os.path.join(ROOT, "include", "s1_executor.h")]):
+        subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-I" + sysconfig.get_paths()["include"],
+                        "-I" + os.path.join(ROOT, "include"), "-o", out, src], check=True)
     return out
 
 

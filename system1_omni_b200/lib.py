@@ -210,8 +210,21 @@ def load(path=None):
     version = lib.cs1_abi_version()
     if version != ABI_VERSION:
         raise RuntimeError(f"{path} has ABI version {version}, expected {ABI_VERSION}")
+    _bind_directly(lib)
     _LIB = lib
     return lib
+
+
+def _bind_directly(lib):
+    """Calls of the step operators with plain numbers go past ctypes, which would take longer to convert their
+    arguments than the operators take to run; with anything else they are the ctypes functions they replace."""
+    try:
+        from . import _fastcall
+    except ImportError:
+        return
+    for name in _fastcall.NAMES:
+        fn = getattr(lib, name)
+        setattr(lib, name, _fastcall.bind(name, C.cast(fn, C.c_void_p).value, fn))
 
 
 def error_string(code):

@@ -286,3 +286,30 @@ def copy(cs1, pools=(A, 2 * A), n_pages=8, page_bytes=32, src=(0, 1), dst=(4, 5)
                                  dict(src=(3, 1), dst=(3, 2))])
 def test_page_copies_refuse(cs1, bad):
     assert copy(cs1, **bad) == INVALID
+
+
+def test_direct_calls_answer_as_ctypes_does(cs1):
+    """Plain numbers go straight to the library, everything else through ctypes: the same answers and errors."""
+    from system1_omni_b200 import _fastcall
+    assert set(_fastcall.NAMES) == {"s1_gdn_step", "s1_gdn_conv_gates_step", "s1_attn_prep_paged", "s1_attention_paged", "s1_pages_copy"}
+    for name in _fastcall.NAMES:
+        assert type(getattr(cs1, name)).__name__ == "Bound"
+    f = cs1.s1_gdn_step
+    plain = [A, A, A, A, A, A, 4, 4, 2, 1.0, A, 4, 4 * 16384, None, A, A, 0, None]
+    assert f(*plain) == 0                                               # no sequences
+    for i in (0, 9, 10, 13, 17):                                        # another kind of argument at one place
+        a = list(plain)
+        a[i] = C.c_void_p(a[i]) if i != 9 else 1
+        assert f(*a) == 0
+    bad = list(plain)
+    bad[7] = 0                                                          # H
+    assert f(*bad) == INVALID
+    bad[0] = C.c_void_p(A)
+    assert f(*bad) == INVALID
+    for args in ([], plain[:-1], [object()] + plain[1:], plain[:6] + ["4"] + plain[7:]):
+        with pytest.raises((TypeError, C.ArgumentError)):
+            f(*args)
+    wide = list(plain)
+    wide[16] = 1 << 32                                                  # ctypes keeps the low 32 bits of an int: nseq 0
+    assert f(*wide) == 0
+    assert f(*plain[:6], True, *plain[7:]) == 0
