@@ -52,59 +52,67 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __g
     constexpr int LANES = DH / 8, UNITS = PREP_THREADS / LANES;
     grid_dep_trigger();
     grid_dep_sync();
+    // A row is a few hundred instructions behind three trips to memory, so whatever does not depend on an
+    // earlier trip is asked for at once: row, weights and positions, then page and rotary rows, then the rest.
     const int r = blockIdx.x, tid = threadIdx.x;
+    const int unit0 = blockIdx.y * UNITS;
+    const int heads = a.Hq + 2 * a.Hk;
+    const int unit = min(unit0 + tid / LANES, heads - 1);
+    const bool live = unit0 + tid / LANES < heads, writes = unit0 + UNITS > a.Hq;
+    const int d0 = tid % LANES * 8;
+    const bool is_q = unit < a.Hq, is_v = unit >= a.Hq + a.Hk;
+    const int h = is_q ? unit : is_v ? unit - a.Hq - a.Hk : unit - a.Hq;
+    const bf16* src = is_q ? a.qg + (size_t)r * a.ld + (size_t)h * 2 * DH : (is_v ? a.vr : a.kr) + (size_t)r * a.ld + (size_t)h * DH;
+    const uint4 raw = ld16_stream(src + d0), weight = ld16((is_q ? a.qw : a.kw) + d0);
+    const uint4 gate = is_q ? ld16_stream(src + DH + d0) : make_uint4(0, 0, 0, 0);
     const int p = a.pos[r], sq = a.seq ? a.seq[r] : r;
-    if (p < 0) return;  // the row sits out
     const int turn = a.angle ? a.angle[r] : p;
-    const int slot = p / a.table.page_tokens, off = p - slot * a.table.page_tokens;
+    const int pt = a.table.page_tokens;
+    auto place_of = [&](int row, int pos, int& seq) {  // entry of the page table, -1: the table has none
+        seq = a.seq ? a.seq[row] : row;
+        return pos >= 0 && seq >= 0 && seq < a.table.sequences && pos / pt < a.table.width ? pos / pt : -1;
+    };
+    int pj = writes && tid < a.rows ? a.pos[tid] : -1;
+    if (p < 0) return;  // the row sits out
+    const int slot = p / pt, off = p - slot * pt;
     int code = 0, page = -1;
     if (sq < 0 || sq >= a.table.sequences || slot >= a.table.width)
         code = PAGED_BAD_ROW;
     else if (turn < 0 || turn >= a.angles)
         code = PAGED_BAD_ANGLE;
-    else {
+    else
         page = a.table.pages[(size_t)sq * a.table.width + slot];
-        if (page < 0 || page >= a.table.n_pages) code = PAGED_BAD_PAGE;
+    const int rot = 2 * a.half;
+    uint4 turns[2] = {};
+    if (d0 < rot && code == 0) {
+        // half is a multiple of 8, so the 8 dims of a lane share one aligned table pack
+        turns[0] = ld16(a.cos + (size_t)turn * a.half + d0 % a.half);
+        turns[1] = ld16(a.sin + (size_t)turn * a.half + d0 % a.half);
     }
+    // Two rows at one place of the cache would race: neither is written.
+    bool clash = false;
+    for (int j = tid; writes && j < a.rows; j += PREP_THREADS) {
+        if (j != tid) pj = a.pos[j];
+        if (j == r || pj < 0 || pj % pt != off) continue;
+        int sj;
+        const int slot_j = place_of(j, pj, sj);
+        clash |= slot_j >= 0 && a.table.pages[(size_t)sj * a.table.width + slot_j] == page;
+    }
+    if (code == 0 && (page < 0 || page >= a.table.n_pages)) code = PAGED_BAD_PAGE;
     if (code) {
         if (tid == 0) atomicCAS(a.error, 0, code);
         return;
     }
-    const int unit0 = blockIdx.y * UNITS;
-    const int heads = a.Hq + 2 * a.Hk;
-    const int unit = min(unit0 + tid / LANES, heads - 1);
-    const bool live = unit0 + tid / LANES < heads;
-    const int d0 = tid % LANES * 8;
-    const bool is_q = unit < a.Hq, is_v = unit >= a.Hq + a.Hk;
-    const int h = is_q ? unit : is_v ? unit - a.Hq - a.Hk : unit - a.Hq;
-    const bf16* src = is_q ? a.qg + (size_t)r * a.ld + (size_t)h * 2 * DH : (is_v ? a.vr : a.kr) + (size_t)r * a.ld + (size_t)h * DH;
-    const uint4 raw = ld16_stream(src + d0);
-
-    // Two rows at one place of the cache would race: neither is written.
-    if (unit0 + UNITS > a.Hq) {
-        bool clash = false;
-        for (int j = tid; j < a.rows; j += PREP_THREADS) {
-            const int pj = a.pos[j];
-            if (j == r || pj < 0 || pj % a.table.page_tokens != off) continue;
-            const int sj = a.seq ? a.seq[j] : j, slot_j = pj / a.table.page_tokens;
-            if (sj < 0 || sj >= a.table.sequences || slot_j >= a.table.width) continue;
-            clash |= a.table.pages[(size_t)sj * a.table.width + slot_j] == page;
-        }
-        if (__syncthreads_or(clash)) {
-            if (tid == 0) atomicCAS(a.error, 0, PAGED_CLASH);
-            page = -1;
-        }
+    if (writes && __syncthreads_or(clash)) {
+        if (tid == 0) atomicCAS(a.error, 0, PAGED_CLASH);
+        page = -1;
     }
 
     float x[8], wv[8], y[8], cs[8], sn[8];
     unpack8(raw, x);
-    unpack8(ld16((is_q ? a.qw : a.kw) + d0), wv);
-    const int rot = 2 * a.half;
-    if (d0 < rot) {
-        // half is a multiple of 8, so the 8 dims of a lane share one aligned table pack
-        unpack8(ld16(a.cos + (size_t)turn * a.half + d0 % a.half), cs);
-        unpack8(ld16(a.sin + (size_t)turn * a.half + d0 % a.half), sn);
-    }
+    unpack8(weight, wv);
+    unpack8(turns[0], cs);
+    unpack8(turns[1], sn);
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i++) ss += x[i] * x[i];
@@ -120,7 +128,7 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __g
     if (!live) return;
     if (is_q) {
         st16(a.q + ((size_t)r * a.Hq + h) * DH + d0, pack8(y));
-        st16(a.gate + ((size_t)r * a.Hq + h) * DH + d0, ld16_stream(src + DH + d0));
+        st16(a.gate + ((size_t)r * a.Hq + h) * DH + d0, gate);
     } else if (page >= 0) {
         const size_t at = (((size_t)page * a.table.page_tokens + off) * a.Hk + h) * DH + d0;
         if (is_v)
@@ -327,11 +335,13 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
     if (warp == CONSUMERS) {
         // ---- copies: the whole warp walks, lane b looks up the page of box b and issues its copies ----
         const uint64_t once = policy_evict_first();
+        int4 note = make_int4(-1, 0, 0, 0);  // row and unit that begin here and go on, the block of their last part
         uint32_t it = 0;
         while (w.left > 0) {
             const int n = a.len[w.row], sq = a.seq ? a.seq[w.row] : w.row;
             const int* pages = a.table.pages + (size_t)sq * a.table.width;
             const int column = w.unit / a.chunks * (HB * DH / 64);
+            const int from = w.tile;
             const int end = (int)min((long long)w.tiles, w.tile + w.left);
             for (; w.tile < end; w.tile++, w.left--, it++) {
                 const int stage = it % G::STAGES;
@@ -361,7 +371,24 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                     tma_load_3d(dst + G::KV_BYTES, &maps.v, 0, at, column, &full[stage], once);
                 }
             }
+            if (end < w.tiles && from == 0) {
+                // it begins here, ends this run and goes on: its last tile lies that far behind the run's end
+                const Cut cut = whole_cut;
+                note = make_int4(w.row, w.unit, cut.run_of(cut.begin(blockIdx.x + 1) + w.tiles - end - 1), 0);
+            }
             if (w.left > 0) walk_next_piece<TILE>(a, w);
+        }
+        if (lane == 0) reinterpret_cast<int4*>(a.work + (size_t)gridDim.x * 2 * part_floats(HB * a.chunk, DH))[blockIdx.x] = note;
+        // rows without tiles: an empty one has nothing to attend to and gets zeros
+        for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+            const int n = a.len[r], sq = a.seq ? a.seq[r] : r;
+            if (n < 0) continue;
+            if (sq < 0 || sq >= a.table.sequences || n > (long long)a.table.width * a.table.page_tokens) {
+                if (lane == 0) fail(PAGED_BAD_ROW);
+            } else if (n == 0) {
+                uint32_t* z = reinterpret_cast<uint32_t*>(a.out + (size_t)r * a.Hq * DH);
+                for (int i = lane; i < a.Hq * DH / 2; i += 32) z[i] = 0;
+            }
         }
     } else {
         constexpr int NT = DH / 8;                          // n-tiles of 8 dims of the result
@@ -373,7 +400,6 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
         const int k_tok = (lane >> 4) * 8 + (lane & 7), k_ch = (lane >> 3) & 1;
         const int v_tok = lane & 15, v_ch = lane >> 4;
         const uint32_t my_tiles = sub * BOX_BYTES + mine * (DH / 64) * (SLICE * 128);
-        int4 note = make_int4(-1, 0, 0, 0);  // row and unit that begin here and go on, the block of their last part
         uint32_t it = 0;
         bool ok = true;
         while (w.left > 0) {
@@ -552,25 +578,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                     if (rb < heads) pair[rb] = make_float2(mb, lb);
                 }
             }
-            if (from == 0 && !whole) {
-                // it ends this run, and its last tile lies that far behind the run's end
-                const Cut cut = whole_cut;
-                note = make_int4(w.row, w.unit, cut.run_of(cut.begin(blockIdx.x + 1) + w.tiles - end - 1), 0);
-            }
             if (w.left > 0) walk_next_piece<TILE>(a, w);
-        }
-        if (tid == 0)
-            reinterpret_cast<int4*>(a.work + (size_t)gridDim.x * 2 * part_floats(HB * a.chunk, DH))[blockIdx.x] = note;
-    }
-    // rows without tiles: an empty one has nothing to attend to and gets zeros
-    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const int n = a.len[r], sq = a.seq ? a.seq[r] : r;
-        if (n < 0) continue;
-        if (sq < 0 || sq >= a.table.sequences || n > (long long)a.table.width * a.table.page_tokens) {
-            if (tid == 0) atomicCAS(a.error, 0, PAGED_BAD_ROW);
-        } else if (n == 0) {
-            uint32_t* z = reinterpret_cast<uint32_t*>(a.out + (size_t)r * a.Hq * DH);
-            for (int i = tid; i < a.Hq * DH / 2; i += PAGED_THREADS) z[i] = 0;
         }
     }
     // after an abort give copies in flight time to land before the shared memory is released
@@ -757,7 +765,7 @@ extern "C" int s1_attn_prep_paged(const void* qg, const void* kr, const void* vr
                                   void* k_pages, void* v_pages, int n_pages, int page_tokens, const int* table,
                                   int table_pages, int n_seqs, const int* seq, const int* pos, int rows, int Hq, int Hk,
                                   int Dh, int half, float eps, void* stream) {
-    if ((Dh != 128 && Dh != 256) || Hq <= 0 || Hk <= 0 || Hq > (1 << 20) || Hk > (1 << 20) || rows < 0 || angles < 0 || ld % 8 != 0 ||
+    if ((Dh != 128 && Dh != 256) || Hq <= 0 || Hk <= 0 || Hq > (1 << 20) || Hk > (1 << 20) || rows < 0 || rows > 65536 || angles < 0 || ld % 8 != 0 ||
         ld < 2LL * Hq * Dh || ld < (long long)Hk * Dh)
         return cudaErrorInvalidValue;
     // the lane ^ (half / 8) partner exchange needs half a multiple of 8, half / 8 a power of two, 2 * half <= Dh

@@ -55,25 +55,27 @@ __device__ __forceinline__ void unpack4(uint2 p, float (&x)[4]) {
 // HBM bounds it with one token a sequence: 64 KiB of state in, 64 KiB out per head, all of a block's reads
 // issued at once. Measured at 193 sequences of 48 heads (1.22 GB): 187 us, 6.53 TB/s; columns per warp and
 // blocks per SM at least: 32 and 2: 189 us, 16 and 2: 228, 8 and 2: 276 (narrower warps fetch pieces of lines).
-constexpr int CW = 32, CHUNK = 8;
+constexpr int CW = 32, CHUNK = 8, FEW_HEADS = 296;
 
-__global__ void __launch_bounds__(D / CW * 32, 3)
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 12)
     gdn_step_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
                     const float* __restrict__ g, const bf16* __restrict__ beta, bf16* __restrict__ o, int H, int group,
                     float scale, float* states, size_t slot_stride, const StepSeqs seqs, int* error) {
     constexpr int CL = CW / 4, RG = 32 / CL, RL = D / RG;  // lanes over columns, groups of lanes over keys, keys per lane
-    constexpr int WARPS = D / CW;
+    constexpr int SPLIT = D / CW / WARPS;  // blocks of a (sequence, head)
     __shared__ __align__(16) float4 kkqq[CHUNK][D];  // k, k, q, q
     __shared__ __align__(16) uint2 vs[CHUNK][D / 4];
     __shared__ float4 gates[CHUNK];                  // e^g, beta, q.k
     grid_dep_trigger();
     grid_dep_sync();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = (int)(blockIdx.x % H), i = (int)(blockIdx.x / H);
+    const int h = (int)(blockIdx.x / SPLIT % H), i = (int)(blockIdx.x / SPLIT / H);
     const StepSeq sq = step_sequence(seqs, i);
     if (sq.code && threadIdx.x == 0) atomicCAS(error, 0, sq.code);
     if (sq.rows < 0) return;
-    const int c0 = warp * CW + lane % CL * 4, r0 = lane / CL;
+    const int c0 = ((int)(blockIdx.x % SPLIT) * WARPS + warp) * CW + lane % CL * 4, r0 = lane / CL;
+    const int hk = h / group, HK = H / group;
 
     ulonglong2 S[RL];
     if (sq.in >= 0) {
@@ -90,7 +92,6 @@ __global__ void __launch_bounds__(D / CW * 32, 3)
         return;
     }
 
-    const int hk = h / group, HK = H / group;
 #pragma unroll 1
     for (int t0 = 0; t0 < sq.rows; t0 += CHUNK) {
         const int nt = min(CHUNK, sq.rows - t0);
@@ -180,6 +181,10 @@ __global__ void __launch_bounds__(D / CW * 32, 3)
 // y_t = silu(sum_j w_j x_{t-3+j}) per channel, the rows before a sequence's first out of its slot's
 // tail [3, channels] (x_{-3}, x_{-2}, x_{-1}, before the convolution). A thread walks the window's rows
 // for 8 channels with the three rows before in registers; the last row of blocks computes the gates.
+//
+// Bound by the latency of its three trips (slots, rows, results) and by issue slots, some 400 instructions a
+// warp. Measured at 193 sequences of 10240 channels (32 MB, 4.8 us of HBM): 8.1 us; 2, 3 and 4 sequences per
+// block, which load the weights once, 8.1, 9.3 and 8.0. One sequence: 2.2 us.
 constexpr int CONV_THREADS = 128;
 
 __global__ void __launch_bounds__(CONV_THREADS)
@@ -188,22 +193,36 @@ __global__ void __launch_bounds__(CONV_THREADS)
                                const bf16* __restrict__ b, const bf16* __restrict__ a, const bf16* __restrict__ A_log,
                                const bf16* __restrict__ dt_bias, bf16* __restrict__ beta, float* __restrict__ g, int H,
                                bf16* tails, size_t slot_stride, const StepSeqs seqs, int* error) {
+    __shared__ bool clashes[CONV_THREADS / 32];
     grid_dep_trigger();
     grid_dep_sync();
+    const int channels = 2 * key_dim + value_dim;
+    const int c0 = ((int)blockIdx.x * CONV_THREADS + (int)threadIdx.x) * 8;
+    const bool conv = (int)blockIdx.x < conv_blocks && c0 < channels;
+    // weights, kept rows and the first new row are all asked for before anything waits
+    uint4 wraw[4] = {}, x[4] = {};
+    if (conv) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) wraw[j] = ld16(w + (size_t)c0 * 4 + j * 8);
+    }
     const int i = blockIdx.y;
     const StepSeq sq = step_sequence(seqs, i);
     if (sq.code && threadIdx.x == 0) atomicCAS(error, 0, sq.code);
     if (sq.rows < 0) return;
-    const int channels = 2 * key_dim + value_dim;
-    const int c0 = ((int)blockIdx.x * CONV_THREADS + (int)threadIdx.x) * 8;
-    const bool conv = (int)blockIdx.x < conv_blocks && c0 < channels;
-    uint4 x[3] = {};
-    if (conv && sq.in >= 0) {
-        const bf16* src = tails + (size_t)sq.in * slot_stride + c0;
+    if (conv) {
+        if (sq.in >= 0) {
+            const bf16* src = tails + (size_t)sq.in * slot_stride + c0;
 #pragma unroll
-        for (int j = 0; j < 3; j++) x[j] = ld16(src + (size_t)j * channels);
+            for (int j = 0; j < 3; j++) x[j] = ld16(src + (size_t)j * channels);
+        }
+        if (sq.rows > 0) x[3] = ld16_stream(qkv + (size_t)sq.row0 * ld + c0);
     }
-    if (__syncthreads_or(step_clash(seqs, i, sq.in, sq.out, threadIdx.x, CONV_THREADS))) {
+    bool clash = __any_sync(0xffffffffu, step_clash(seqs, i, sq.in, sq.out, threadIdx.x, CONV_THREADS));
+    if ((threadIdx.x & 31) == 0) clashes[threadIdx.x >> 5] = clash;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < CONV_THREADS / 32; j++) clash |= clashes[j];
+    if (clash) {
         if (threadIdx.x == 0) atomicCAS(error, 0, STEP_SLOT_CLASH);
         return;
     }
@@ -219,15 +238,12 @@ __global__ void __launch_bounds__(CONV_THREADS)
     }
     if (!conv) return;
     float wf[8][4];
-    {
-        const bf16* wp = w + (size_t)c0 * 4;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float tmp[8];
-            unpack8(ld16(wp + j * 8), tmp);
+    for (int j = 0; j < 4; j++) {
+        float tmp[8];
+        unpack8(wraw[j], tmp);
 #pragma unroll
-            for (int e = 0; e < 8; e++) wf[(j * 8 + e) / 4][(j * 8 + e) % 4] = tmp[e];
-        }
+        for (int e = 0; e < 8; e++) wf[(j * 8 + e) / 4][(j * 8 + e) % 4] = tmp[e];
     }
     bf16* dst;
     int dld, dc;
@@ -237,14 +253,15 @@ __global__ void __launch_bounds__(CONV_THREADS)
         dst = k, dld = key_dim, dc = c0 - key_dim;
     else
         dst = v, dld = value_dim, dc = c0 - 2 * key_dim;
+#pragma unroll 1
     for (int t = 0; t < sq.rows; t++) {
         const size_t row = (size_t)sq.row0 + t;
-        const uint4 now = ld16_stream(qkv + row * ld + c0);
+        if (t > 0) x[3] = ld16_stream(qkv + row * ld + c0);
         float x0[8], x1[8], x2[8], x3[8], y[8];
         unpack8(x[0], x0);
         unpack8(x[1], x1);
         unpack8(x[2], x2);
-        unpack8(now, x3);
+        unpack8(x[3], x3);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             float acc = wf[e][0] * x0[e];
@@ -256,7 +273,7 @@ __global__ void __launch_bounds__(CONV_THREADS)
         st16(dst + row * dld + dc, pack8(y));
         x[0] = x[1];
         x[1] = x[2];
-        x[2] = now;
+        x[2] = x[3];
     }
     bf16* keep = tails + (size_t)sq.out * slot_stride + c0;
 #pragma unroll
@@ -295,13 +312,15 @@ extern "C" int s1_gdn_step(const void* q, const void* k, const void* v, const fl
     if (!states || !aligned16(states)) return cudaErrorInvalidValue;
     if (rows > 0 && (!q || !k || !v || !g || !beta || !o || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)))
         return cudaErrorInvalidValue;
-    const long long blocks = (long long)nseq * H;
-    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    // few heads to step: a block per warp's columns, so that four times as many SMs take part (32 heads: 3.9 us for 4.4)
+    const long long heads = (long long)nseq * H;
+    if (heads > 0x7fffffffLL / 4) return cudaErrorInvalidValue;
+    const bool few = heads <= FEW_HEADS;
     int* error = nullptr;
     const int rc = error_word(&error);
     if (rc != 0) return rc;
     const cudaError_t e =
-        launch_dep(gdn_step_kernel, (unsigned)blocks, D / CW * 32, 0, as_stream(stream), static_cast<const bf16*>(q),
+        launch_dep(few ? gdn_step_kernel<1> : gdn_step_kernel<4>, (unsigned)(few ? 4 * heads : heads), few ? 32 : 128, 0, as_stream(stream), static_cast<const bf16*>(q),
                    static_cast<const bf16*>(k), static_cast<const bf16*>(v), g, static_cast<const bf16*>(beta),
                    static_cast<bf16*>(o), H, H / HK, scale, states, slot_stride, seqs, error);
     return e != cudaSuccess ? e : cudaGetLastError();
