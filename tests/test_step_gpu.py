@@ -793,3 +793,112 @@ def test_two_attentions_at_once_on_their_own_workspaces(cs1, stream):
                                            c["table"].shape[1], 6, None, ln.at(), 6, 24, 4, 128, 128 ** -0.5, ws.at(), floats, st.handle), "attention")
     for st, w, s in zip(sts, want, state):
         assert (down(s[3], w.shape, st) == w).all()
+
+
+def test_layer_steps_continue_its_prefill(cs1, stream):
+    """One Gated DeltaNet layer: prompts of several lengths, then tokens one at a time and a window of them, from their
+    slots and from a shared one, against the oracle's layer on the whole sequences."""
+    from system1_omni_b200.gdn_layer import GdnLayer
+    from test_gdn_layer_gpu import make_case, oracle_layer, rel_l2
+    hidden, hk, hv = 1024, 4, 8
+    prompts, more = [70, 2, 64, 1], 5
+    total = [n + more for n in prompts]
+    layer = GdnLayer(hidden, hk, hv, max_tokens=128, stream=stream, slots=7)
+    try:
+        xs = [make_case(n, hidden, hk, hv, seed=i)[0] for i, n in enumerate(total)]
+        w = make_case(1, hidden, hk, hv)[1]
+        layer.set_weights(**w)
+        for slot, (n, x) in enumerate(zip(prompts, xs)):
+            x_dev = up(x[:n], stream)
+            layer.forward(x_dev.at(), n, slot=slot)
+            stream.sync()
+        got = [np.zeros((more, hidden), np.float32) for _ in prompts]
+        slots = ints([0, 1, 2, 3], stream)
+        for t in range(more - 3):
+            x_dev = up(np.stack([x[n + t] for n, x in zip(prompts, xs)]), stream)
+            y = f32(down(layer.step(x_dev.at(), 4, slots.at(), slots.at(), 4), (128, hidden), stream))
+            for i in range(4):
+                got[i][t] = y[i]
+        # the last three tokens of each as one window; two more sequences begin where the first one stands
+        rows = np.concatenate([x[-3:] for x in xs] + [xs[0][-3:-1], xs[0][-3:-2]])
+        start, si, so = ints([0, 3, 6, 9, 12, 14, 15], stream), ints([0, 1, 2, 3, 0, 0], stream), ints([4, 1, 2, 3, 5, 6], stream)
+        x_dev = up(rows, stream)
+        y = f32(down(layer.step(x_dev.at(), 15, si.at(), so.at(), 6, start.at()), (128, hidden), stream))
+        for i in range(4):
+            got[i][-3:] = y[3 * i:3 * i + 3]
+            want = f32(oracle_layer(xs[i], w, total[i], hidden, hk, hv, float64_core=True))[-more:]
+            # bf16 activations with float32 accumulation on both sides: the gate of the layer's prefill
+            assert rel_l2(got[i], want) < 2e-2, i
+            assert np.abs(got[i] - want).max() < 5e-2 * np.abs(want).max()
+        # the candidates' rows are those of the first sequence, up to the row counts' summation order in the projections
+        assert rel_l2(y[12:14], y[0:2]) < 1e-2 and rel_l2(y[14:15], y[0:1]) < 1e-2
+        with pytest.raises(ValueError):
+            layer.forward(x_dev.at(), 3, slot=7)
+    finally:
+        layer.close()
+
+
+@pytest.mark.parametrize("Dh,page", [(128, 16), (256, 32)])
+def test_candidates_of_a_prefix_in_a_paged_cache(cs1, stream, Dh, page):
+    """A prompt written to pages, forked for three candidates whose tokens follow one at a time, a page copied when a
+    shared one is written, the pool compacted in between: each row against the prefill's attention over the same rows."""
+    from system1_omni_b200.pages import Pages, copy
+    Hq, Hk, half, eps, T, more = 8, 4, 32, 1e-6, 75, 20
+    n_pages, wide = 40, 8
+    angles = T + more
+    common = prep_inputs(T, Hq, Hk, Dh, half, angles, n_pages, page, 0, 1)
+    tails = [prep_inputs(more, Hq, Hk, Dh, half, angles, 1, page, 0, 10 + i) for i in range(3)]
+    d = {m: up(common[m], stream) for m in ("qw", "kw", "cos", "sin", "kp", "vp")}
+    ld, kr, page_bytes = common["ld"], 4 * Hq * Dh, page * Hk * Dh * 2
+    floats = cs1.s1_attention_paged_workspace_floats(Hq, Hk, Dh)
+    ws = L.DeviceBuffer(floats * 4)
+    p = Pages(n_pages, page, 4, wide)
+    try:
+        def step(x, seq, pos):
+            """New rows x at places (seq, pos): written to the cache and attended over it."""
+            rows = len(x)
+            table, _ = p.table()
+            x, table = up(x, stream), up(table, stream)
+            s, q_pos, n = ints(seq, stream), ints(pos, stream), ints([t + 1 for t in pos], stream)
+            q, gate, out = (L.DeviceBuffer(rows * Hq * Dh * 2) for _ in range(3))
+            L.check(cs1.s1_attn_prep_paged(x.at(), x.at(kr), x.at(kr + 2 * Hk * Dh), ld, d["qw"].at(), d["kw"].at(), d["cos"].at(), d["sin"].at(),
+                                           angles, None, q.at(), gate.at(), d["kp"].at(), d["vp"].at(), n_pages, page, table.at(), wide, 4,
+                                           s.at(), q_pos.at(), rows, Hq, Hk, Dh, half, eps, stream.handle), "prep")
+            L.check(cs1.s1_attention_paged(q.at(), gate.at(), out.at(), d["kp"].at(), d["vp"].at(), n_pages, page, table.at(), wide, 4, s.at(),
+                                           n.at(), rows, Hq, Hk, Dh, Dh ** -0.5, ws.at(), floats, stream.handle), "attention")
+            return down(out, (rows, Hq, Dh), stream)
+
+        assert p.append(0, T) == []
+        got = [step(common["x"], [0] * T, list(range(T)))] + [np.zeros((more, Hq, Dh), np.uint16) for _ in range(3)]
+        for i in range(3):
+            p.fork(0, 1 + i)
+        copies = 0
+        for t in range(more):
+            pairs = sum((p.append(1 + i, 1) for i in range(3)), [])
+            copies += len(pairs)
+            copy([d["kp"].at(), d["vp"].at()], n_pages, page_bytes, pairs, stream)
+            y = step(np.stack([x["x"][t] for x in tails]), [1, 2, 3], [T + t] * 3)
+            for i in range(3):
+                got[1 + i][t] = y[i]
+            if t == 4:
+                p.truncate(0)                   # the prompt alone is not needed any more
+                copy([d["kp"].at(), d["vp"].at()], n_pages, page_bytes, p.compact(), stream)
+        assert copies == 3                      # the half-filled page of the prompt, once per candidate
+        used = n_pages - p.free_pages()
+        assert used == T // page + 3 * -(-(T % page + more) // page) and p.table(1)[0].max() < used + 3
+        for i in range(3):
+            x = np.concatenate([common["x"], tails[i]["x"]])
+            n = T + more
+            dx = up(x, stream)
+            q, gate, k, out = (L.DeviceBuffer(n * h * Dh * 2) for h in (Hq, Hq, Hk, Hq))
+            L.check(cs1.cs1_attn_prep(dx.at(), dx.at(kr), ld, d["qw"].at(), d["kw"].at(), d["cos"].at(), d["sin"].at(), q.at(), gate.at(), k.at(), n, Hq,
+                                      Hk, Dh, half, eps, stream.handle), "prefill prep")
+            L.check(cs1.cs1_attention_gated(q.at(), k.at(), dx.at(kr + 2 * Hk * Dh), ld, gate.at(), out.at(), n, Hq, Hk, Dh, Dh ** -0.5,
+                                            stream.handle), "prefill attention")
+            want = f32(down(out, (n, Hq, Dh), stream)).astype(np.float64)
+            mine = f32(np.concatenate([got[0], got[1 + i]])).astype(np.float64)
+            # the prefill's own gate for its attention against float64, twice: both sides have such an error
+            assert np.abs(mine - want).max() < 2 * 1.6e-2 * np.abs(want).max()
+            assert np.linalg.norm(mine - want) < 2 * 1.6e-2 * np.linalg.norm(want)
+    finally:
+        p.close()
