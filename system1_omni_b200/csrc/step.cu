@@ -53,9 +53,18 @@ __device__ __forceinline__ void unpack4(uint2 p, float (&x)[4]) {
 
 //
 // HBM bounds it with one token a sequence: 64 KiB of state in, 64 KiB out per head, all of a block's reads
-// issued at once. Measured at 193 sequences of 48 heads (1.22 GB): 187 us, 6.53 TB/s; columns per warp and
+// issued at once. Measured at 193 sequences of 48 heads (1.22 GB): 186 us, 6.55 TB/s; columns per warp and
 // blocks per SM at least: 32 and 2: 189 us, 16 and 2: 228, 8 and 2: 276 (narrower warps fetch pieces of lines).
+// Windows are bound by the FMA pipe's latency, a third of its rate, with the three warps per scheduler that such
+// registers leave: 37 windows of 1 to 9 tokens, 32 heads, 38 us (the bytes alone 13). The products of eight
+// tokens at once on the tensor cores with the state split into three bf16 took 39 to 43 us, two resident blocks
+// that prefetch the next state into shared memory 49 to 55.
 constexpr int CW = 32, CHUNK = 8, FEW_HEADS = 296;
+
+__device__ __forceinline__ void copy16(const void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 12)
@@ -65,7 +74,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 12)
     constexpr int CL = CW / 4, RG = 32 / CL, RL = D / RG;  // lanes over columns, groups of lanes over keys, keys per lane
     constexpr int SPLIT = D / CW / WARPS;  // blocks of a (sequence, head)
     __shared__ __align__(16) float4 kkqq[CHUNK][D];  // k, k, q, q
-    __shared__ __align__(16) uint2 vs[CHUNK][D / 4];
+    __shared__ __align__(16) bf16 ks[CHUNK][D], qs[CHUNK][D], vs[CHUNK][D];
     __shared__ float4 gates[CHUNK];                  // e^g, beta, q.k
     grid_dep_trigger();
     grid_dep_sync();
@@ -77,6 +86,24 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 12)
     const int c0 = ((int)(blockIdx.x % SPLIT) * WARPS + warp) * CW + lane % CL * 4, r0 = lane / CL;
     const int hk = h / group, HK = H / group;
 
+    // Rows t0 .. of a chunk as they are. The first ones are asked for before the state, which they would queue behind.
+    float g_mine = 0.f, beta_mine = 0.f;  // of row t0 + threadIdx.x
+    auto fetch = [&](int t0) {
+        const int nt = min(CHUNK, sq.rows - t0);
+        for (int e = threadIdx.x; e < nt * (D / 8); e += WARPS * 32) {
+            const int t = e / (D / 8), d = e % (D / 8) * 8;
+            const size_t row = (size_t)sq.row0 + t0 + t;
+            copy16(&ks[t][d], k + (row * HK + hk) * D + d);
+            copy16(&qs[t][d], q + (row * HK + hk) * D + d);
+            copy16(&vs[t][d], v + (row * H + h) * D + d);
+        }
+        if ((int)threadIdx.x < nt) {
+            const size_t at = ((size_t)sq.row0 + t0 + threadIdx.x) * H + h;
+            g_mine = g[at], beta_mine = f32(beta[at]);
+        }
+    };
+    fetch(0);
+
     ulonglong2 S[RL];
     if (sq.in >= 0) {
         const float* src = states + (size_t)sq.in * slot_stride + ((size_t)h * D + r0) * D + c0;
@@ -87,7 +114,8 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 12)
         for (int j = 0; j < RL; j++) S[j] = make_ulonglong2(0, 0);
     }
     const bool clash = step_clash(seqs, i, sq.in, sq.out, threadIdx.x, WARPS * 32);
-    if (sq.rows == 0 && __syncthreads_or(clash)) {
+    copies_wait();
+    if (__syncthreads_or(clash)) {
         if (threadIdx.x == 0) atomicCAS(error, 0, STEP_SLOT_CLASH);
         return;
     }
@@ -95,17 +123,17 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 12)
 #pragma unroll 1
     for (int t0 = 0; t0 < sq.rows; t0 += CHUNK) {
         const int nt = min(CHUNK, sq.rows - t0);
-        if (t0 > 0) __syncthreads();  // the rows before have been read
+        if (t0 > 0) {
+            __syncthreads();  // the rows before have been read
+            fetch(t0);
+            copies_wait();
+            __syncthreads();
+        }
 #pragma unroll 1
         for (int t = warp; t < nt; t += WARPS) {
-            const size_t row = (size_t)sq.row0 + t0 + t;
-            const uint2 kr = *reinterpret_cast<const uint2*>(k + (row * HK + hk) * D + lane * 4);
-            const uint2 qr = *reinterpret_cast<const uint2*>(q + (row * HK + hk) * D + lane * 4);
-            vs[t][lane] = *reinterpret_cast<const uint2*>(v + (row * H + h) * D + lane * 4);
-            const float gt = g[row * H + h], bt = f32(beta[row * H + h]);
             float kv[4], qv[4];
-            unpack4(kr, kv);
-            unpack4(qr, qv);
+            unpack4(*reinterpret_cast<const uint2*>(&ks[t][lane * 4]), kv);
+            unpack4(*reinterpret_cast<const uint2*>(&qs[t][lane * 4]), qv);
             float kk = 0.f, qq = 0.f, qk = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; e++) kk += kv[e] * kv[e], qq += qv[e] * qv[e], qk += kv[e] * qv[e];
@@ -114,16 +142,10 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 12)
             qk = warp_sum(qk) * kk * qq;
 #pragma unroll
             for (int e = 0; e < 4; e++) kkqq[t][lane * 4 + e] = make_float4(kv[e] * kk, kv[e] * kk, qv[e] * qq, qv[e] * qq);
-            if (lane == 0) gates[t] = make_float4(expf(gt), bt, qk, 0.f);
+            if (lane == 0) gates[t].z = qk;
         }
-        if (t0 == 0) {
-            if (__syncthreads_or(clash)) {
-                if (threadIdx.x == 0) atomicCAS(error, 0, STEP_SLOT_CLASH);
-                return;
-            }
-        } else {
-            __syncthreads();
-        }
+        if ((int)threadIdx.x < nt) gates[threadIdx.x].x = expf(g_mine), gates[threadIdx.x].y = beta_mine;
+        __syncthreads();
 #pragma unroll 1
         for (int t = 0; t < nt; t++) {
             const uint32_t rows_at = (uint32_t)__cvta_generic_to_shared(&kkqq[t][r0]);
@@ -150,7 +172,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 12)
                     qs[e] += __shfl_xor_sync(0xffffffffu, qs[e], m);
                 }
             const float4 gt = gates[t];
-            unpack4(vs[t][c0 / 4], vv);
+            unpack4(*reinterpret_cast<const uint2*>(&vs[t][c0]), vv);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 d[e] = gt.y * (vv[e] - gt.x * ks[e]);
