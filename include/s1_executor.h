@@ -106,7 +106,8 @@ int s1_gdn_conv_gates_batch(const void* qkv, int ld, const void* w, void* q, voi
  * unwritten, with a code in the family's device error word (s1_device_status): 60 rows outside the
  * operands, 61 a slot outside the pool, 62 sequences that would race for a slot (delta-rule family);
  * 31 a row whose sequence or position the table does not have, 32 a page outside the pools, 33 a
- * position outside the rotary tables, 34 rows at one place of the cache (attention family).
+ * position outside the rotary tables, 34 rows at one place of the cache, 30 a bounded wait that ran out
+ * (attention family). A code stays until it is read, and the executor's calls that check the words report it too.
  * The first call of an operator on a GPU looks up the address of that word: make it before any
  * stream capture. All pointers belong to the current device, as everywhere in this interface. */
 
@@ -118,7 +119,7 @@ int s1_gdn_conv_gates_batch(const void* qkv, int ld, const void* w, void* q, voi
  * 4, at least H * 128 * 128), each [H, 128 (key), 128 (value)] as s_in / s_out there. slot_in[i] may equal slot_out[i]
  * (update in place) and several sequences may begin with one slot that none of them writes (the
  * candidates of a prefix); a slot that one sequence writes and another one names is refused for
- * both. A sequence without rows copies its state. Float32 throughout. */
+ * both. A sequence without rows copies its state. At most 65535 sequences. Float32 throughout. */
 int s1_gdn_step(const void* q, const void* k, const void* v, const float* g, const void* beta, void* o, int rows, int H,
                 int HK, float scale, float* states, int n_slots, size_t slot_stride, const int* start, const int* slot_in,
                 const int* slot_out, int nseq, void* stream);
@@ -144,7 +145,8 @@ int s1_gdn_conv_gates_step(const void* qkv, int ld, const void* w, void* q, void
  * rows of ld elements; q and gate [rows, Hq, Dh] come out, keys and values go to their places in the cache. The rotary
  * tables cos, sin [angles, half] are read at row angle[r] (null: at pos[r]), so tables of one row per
  * packed row serve positions on several axes. Rows at one place of the cache are refused: their q
- * and gate come out, the place is left as it is. Any page_tokens; 16-byte aligned pointers. */
+ * and gate come out, the place is left as it is. Any page_tokens; 16-byte aligned pointers; at most
+ * 65536 rows (each is compared with every other). */
 int s1_attn_prep_paged(const void* qg, const void* kr, const void* vr, int ld, const void* qw, const void* kw,
                        const void* cos, const void* sin, int angles, const int* angle, void* q, void* gate, void* k_pages,
                        void* v_pages, int n_pages, int page_tokens, const int* table, int table_pages, int n_seqs,

@@ -46,7 +46,8 @@ struct PrepArgs {
 constexpr int PREP_THREADS = 256;
 
 // DH / 8 lanes per head, 8 consecutive dims per lane; the rotary partner of dim d (d +- half) lives
-// half / 8 lanes away. A row's units are its Hq query heads, Hk key heads and Hk value heads.
+// half / 8 lanes away. A row's units are its Hq query heads, Hk key heads and Hk value heads. Latency bounds it:
+// 251 rows of 16 and 4 heads of 256 (10 MB) take 5.2 us, one row 2.3, launch and all.
 template <int DH>
 __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __grid_constant__ PrepArgs a) {
     constexpr int LANES = DH / 8, UNITS = PREP_THREADS / LANES;
@@ -156,6 +157,12 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __g
 // cut into equal runs, one per block, whatever the lengths are. A run's pieces that cover a (row, head
 // block) whole are finished by the block; the others leave maximum, sum and weighted values in
 // float32 in the workspace, and a second kernel joins the parts of each in order.
+//
+// Measured, in a recorded graph: 65 caches of 500 to 16000 tokens, 24 query and 4 key-value heads of 128
+// (630 MB): 104 us, 6.1 TB/s with the join; 250001 tokens, 16 and 4 heads of 256 (1.02 GB): 159 us, 6.4 TB/s;
+// 1500 tokens: 9.2 us, of which the join is 3.6. Before, tiles of 64 tokens of one head whose warps shared
+// every tile's maximum and probabilities: 119 (one block per SM), 113 us (two). The first kernel alone takes 100 us:
+// what is left is its start (3 us to the first tile) and the join.
 constexpr int CONSUMERS = 4, PAGED_THREADS = (CONSUMERS + 1) * 32;
 constexpr int SLICE = 16;       // tokens of a warp's part of a tile, and of a copied box
 constexpr int MIN_RUN = 2;      // tiles: a run of one saves nothing and leaves twice the parts to join

@@ -2,7 +2,7 @@
 // write, fork, truncate, compact). Plain bookkeeping, no device calls; the copies that it asks for
 // are s1_pages_copy's.
 #include <algorithm>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "s1_executor.h"
@@ -46,7 +46,7 @@ extern "C" int s1_pages_create(int n_pages, int page_tokens, int max_seqs, int m
         p->users.assign(n_pages, 0);
         p->seq.resize(max_seqs);
         p->tokens.assign(max_seqs, 0);
-    } catch (const std::bad_alloc&) {
+    } catch (const std::exception&) {
         delete of(*pages);
         *pages = nullptr;
         return S1_ERR_PAGES;
@@ -67,7 +67,7 @@ extern "C" int s1_pages_append(void* pages, int seq, int tokens, int* src, int* 
     if (need > p->max_seq_pages || need - (long long)own.size() + copy > (long long)p->free.size() || (copy && cap < 1)) return S1_ERR_PAGES;
     try {
         own.reserve((size_t)need);
-    } catch (const std::bad_alloc&) {
+    } catch (const std::exception&) {
         return S1_ERR_PAGES;
     }
     *n_copies = copy;
@@ -86,7 +86,7 @@ extern "C" int s1_pages_fork(void* pages, int from, int to) {
     if (!p || !p->has(from) || !p->has(to) || from == to || !p->seq[to].empty()) return S1_ERR_ARGUMENT;
     try {
         p->seq[to] = p->seq[from];
-    } catch (const std::bad_alloc&) {
+    } catch (const std::exception&) {
         p->seq[to].clear();
         return S1_ERR_PAGES;
     }
@@ -119,7 +119,7 @@ extern "C" int s1_pages_compact(void* pages, int* src, int* dst, int cap, int* n
     std::vector<int> place;
     try {
         place.assign(total, -1);
-    } catch (const std::bad_alloc&) {
+    } catch (const std::exception&) {
         return S1_ERR_PAGES;
     }
     *n_copies = moves;

@@ -51,7 +51,6 @@ __device__ __forceinline__ void unpack4(uint2 p, float (&x)[4]) {
     x[2] = __uint_as_float(p.y << 16), x[3] = __uint_as_float(p.y & 0xffff0000u);
 }
 
-//
 // HBM bounds it with one token a sequence: 64 KiB of state in, 64 KiB out per head, all of a block's reads
 // issued at once. Measured at 193 sequences of 48 heads (1.22 GB): 186 us, 6.55 TB/s; columns per warp and
 // blocks per SM at least: 32 and 2: 189 us, 16 and 2: 228, 8 and 2: 276 (narrower warps fetch pieces of lines).
@@ -357,7 +356,7 @@ extern "C" int s1_gdn_conv_gates_step(const void* qkv, int ld, const void* w, vo
         (long long)ld < 2LL * key_dim + value_dim || ld < H || 2LL * key_dim + value_dim > 0x7fffffffLL)
         return cudaErrorInvalidValue;
     const int channels = 2 * key_dim + value_dim;
-    if (slot_stride < 3 * (size_t)channels || slot_stride % 8 != 0 || (long long)rows * H > 0x7fffffffLL || nseq > 65535)
+    if (slot_stride < 3 * (size_t)channels || slot_stride % 8 != 0 || (long long)rows * H > 0x7fffffffLL)
         return cudaErrorInvalidValue;
     if (nseq == 0) return cudaSuccess;
     if (!tails || !aligned16(tails) || !w || !aligned16(w) || !A_log || !dt_bias) return cudaErrorInvalidValue;

@@ -47,8 +47,9 @@ __device__ __forceinline__ bool step_clash(const StepSeqs& s, int i, int in, int
     return clash;
 }
 
+// (At most 65535 sequences: a grid dimension, and every sequence is compared with every other.)
 inline bool step_seqs_ok(const StepSeqs& s) {
-    return s.nseq >= 0 && s.rows >= 0 && s.n_slots >= 0 && (s.nseq == 0 || (s.slot_in && s.slot_out));
+    return s.nseq >= 0 && s.nseq <= 65535 && s.rows >= 0 && s.n_slots >= 0 && (s.nseq == 0 || (s.slot_in && s.slot_out));
 }
 
 }  // namespace s1

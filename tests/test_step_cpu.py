@@ -199,7 +199,7 @@ def step(cs1, **kw):
 @pytest.mark.parametrize("bad", [dict(H=0), dict(HK=0), dict(HK=3), dict(rows=-1), dict(nseq=-1), dict(n_slots=-1), dict(stride=4 * 16384 - 4),
                                  dict(stride=4 * 16384 + 2), dict(si=None), dict(so=None), dict(states=None), dict(states=A + 4),
                                  dict(q=None), dict(k=A + 8), dict(v=A + 2), dict(o=None), dict(g=None), dict(beta=None),
-                                 dict(nseq=1 << 30)])
+                                 dict(nseq=65536), dict(nseq=65535, H=1 << 15, HK=1, stride=(1 << 15) * 16384)])
 def test_delta_rule_step_refuses(cs1, bad):
     assert step(cs1, **bad) == INVALID
 
@@ -239,7 +239,7 @@ def prep(cs1, **kw):
                                   a["rows"], a["Hq"], a["Hk"], a["Dh"], a["half"], 1e-6, None)
 
 
-@pytest.mark.parametrize("bad", [dict(Dh=64), dict(Hq=0), dict(Hk=0), dict(ld=2047), dict(ld=1016), dict(rows=-1), dict(half=0), dict(half=12),
+@pytest.mark.parametrize("bad", [dict(Dh=64), dict(Hq=0), dict(Hk=0), dict(ld=2047), dict(ld=1016), dict(rows=-1), dict(rows=65537), dict(half=0), dict(half=12),
                                  dict(half=24), dict(half=128), dict(angles=-1), dict(n_pages=0), dict(page=0), dict(table=None),
                                  dict(wide=0), dict(seqs=0), dict(pos=None), dict(n_pages=1 << 28), dict(wide=1 << 27), dict(qg=None),
                                  dict(kr=A + 2), dict(vr=None), dict(qw=A + 8), dict(kw=None), dict(cos=None), dict(sin=A + 4),

@@ -902,3 +902,31 @@ def test_candidates_of_a_prefix_in_a_paged_cache(cs1, stream, Dh, page):
             assert np.linalg.norm(mine - want) < 2 * 1.6e-2 * np.linalg.norm(want)
     finally:
         p.close()
+
+
+def test_cache_writes_reach_the_attention_launched_as_its_dependent(cs1, stream):
+    """Prep, then attention over what it just wrote, as programmatic dependents and without: the same bits."""
+    Hq, Hk, Dh, page, rows = 8, 4, 128, 16, 48
+    c = prep_inputs(rows, Hq, Hk, Dh, 16, 64, 30, page, 0, 5)
+    table = make_table([3] * 8, 30, 4, 2)
+    seq, pos = np.arange(rows) % 8, np.arange(rows) // 8
+    kr, floats = 4 * Hq * Dh, cs1.s1_attention_paged_workspace_floats(Hq, Hk, Dh)
+    want = None
+    for mode in (0, 1, 1, 1):
+        d = {m: up(c[m], stream) for m in ("x", "qw", "kw", "cos", "sin", "kp", "vp")}
+        t, s, p, n = ints(table, stream), ints(seq, stream), ints(pos, stream), ints(pos + 1, stream)
+        q, gate, out = (L.DeviceBuffer(rows * Hq * Dh * 2) for _ in range(3))
+        ws = L.DeviceBuffer(floats * 4)
+        stream.sync()
+        before = cs1.s1_set_dependent_launch(mode)
+        for _ in range(8):
+            L.check(cs1.s1_attn_prep_paged(d["x"].at(), d["x"].at(kr), d["x"].at(kr + 2 * Hk * Dh), c["ld"], d["qw"].at(), d["kw"].at(), d["cos"].at(),
+                                           d["sin"].at(), 64, None, q.at(), gate.at(), d["kp"].at(), d["vp"].at(), 30, page, t.at(), 4, 8, s.at(),
+                                           p.at(), rows, Hq, Hk, Dh, 16, 1e-6, stream.handle), "prep")
+            L.check(cs1.s1_attention_paged(q.at(), gate.at(), out.at(), d["kp"].at(), d["vp"].at(), 30, page, t.at(), 4, 8, s.at(), n.at(), rows, Hq,
+                                           Hk, Dh, Dh ** -0.5, ws.at(), floats, stream.handle), "attention")
+        cs1.s1_set_dependent_launch(before)
+        got = down(out, (rows, Hq, Dh), stream)
+        if want is None:
+            want = got
+        assert (got == want).all()
