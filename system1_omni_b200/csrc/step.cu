@@ -66,7 +66,7 @@ __device__ __forceinline__ void copy16(const void* dst, const void* src) {
 __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 template <int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 12)
+__global__ void __launch_bounds__(WARPS * 32, WARPS == 4 ? 3 : 8)
     gdn_step_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k, const bf16* __restrict__ v,
                     const float* __restrict__ g, const bf16* __restrict__ beta, bf16* __restrict__ o, int H, int group,
                     float scale, float* states, size_t slot_stride, const StepSeqs seqs, int* error) {
@@ -333,7 +333,7 @@ extern "C" int s1_gdn_step(const void* q, const void* k, const void* v, const fl
     if (!states || !aligned16(states)) return cudaErrorInvalidValue;
     if (rows > 0 && (!q || !k || !v || !g || !beta || !o || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o)))
         return cudaErrorInvalidValue;
-    // few heads to step: a block per warp's columns, so that four times as many SMs take part (32 heads: 3.9 us for 4.4)
+    // few heads to step: a block per warp's columns, so that four times as many SMs take part (32 heads: 3.3 us for 4.6; from some 600 heads on it is slower)
     const long long heads = (long long)nseq * H;
     if (heads > 0x7fffffffLL / 4) return cudaErrorInvalidValue;
     const bool few = heads <= FEW_HEADS;
