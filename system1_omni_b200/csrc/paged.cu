@@ -160,12 +160,12 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __g
 //
 // Measured, in a recorded graph: 65 caches of 500 to 16000 tokens, 24 query and 4 key-value heads of 128
 // (630 MB): 104 us, 6.1 TB/s with the join; 250001 tokens, 16 and 4 heads of 256 (1.02 GB): 159 us, 6.4 TB/s;
-// 1500 tokens: 9.2 us, of which the join is 3.6. Before, tiles of 64 tokens of one head whose warps shared
-// every tile's maximum and probabilities: 119 (one block per SM), 113 us (two). The first kernel alone takes 100 us:
-// what is left is its start (3 us to the first tile) and the join.
+// 1500 tokens: 9.1 us, of which the join is 3.6; 2 tokens: 7. Before, tiles of 64 tokens of one head whose warps
+// shared every tile's maximum and probabilities: 119 us (one block per SM), 113 (two) for the first. The
+// first kernel alone takes 100 us of it: what is left is its start (2.4 us to the first tile) and the join.
 constexpr int CONSUMERS = 4, PAGED_THREADS = (CONSUMERS + 1) * 32;
 constexpr int SLICE = 16;       // tokens of a warp's part of a tile, and of a copied box
-constexpr int MIN_RUN = 2;      // tiles: a run of one saves nothing and leaves twice the parts to join
+constexpr int MIN_RUN = 1;      // tiles
 constexpr int MAX_GROUP = 16;   // query heads of one key-value head that a block takes at once
 constexpr int MAX_BLOCKS = 296; // two per SM
 
@@ -175,9 +175,12 @@ struct PCfg {
     static constexpr int STAGES = 3;
     static constexpr int KV_BYTES = CONSUMERS * SLICE * DH * 2;
     static constexpr int STAGE = 2 * KV_BYTES;
-    static constexpr int OFF_SUM = STAGES * STAGE;                 // float [HB][16][64] for HB <= 2
-    static constexpr int OFF_ML = OFF_SUM + 2 * 16 * 64 * 4;       // float2 [4][16]
-    static constexpr int OFF_BAR = OFF_ML + CONSUMERS * 16 * 8;
+    static constexpr int PART = DH == 128 ? 32 : 64;              // dims that a warp hands over at a time
+    static constexpr int PITCH = PART + 4;
+    static constexpr int OFF_SUM = STAGES * STAGE;                 // float [4][16][PITCH]
+    static constexpr int OFF_ML = OFF_SUM + CONSUMERS * 16 * PITCH * 4;  // float2 [4][16]
+    static constexpr int OFF_INV = OFF_ML + CONSUMERS * 16 * 8;    // float [HB][16], 1 / sum
+    static constexpr int OFF_BAR = OFF_INV + CONSUMERS * 16 * 4;
     static constexpr int SMEM = OFF_BAR + 2 * STAGES * 8 + 64 + 1024;  // and what aligning the base takes
 };
 
@@ -259,7 +262,26 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-__device__ __forceinline__ float gated(float o, float gate) { return o / (1.f + __expf(-gate)); }
+// The warps of one head meet: all consumers, or the one warp.
+template <int SUBS>
+__device__ __forceinline__ void piece_sync() {
+    if constexpr (SUBS > 1)
+        consumer_sync();
+    else
+        __syncwarp();
+}
+
+// (__fdividef is off by 2^-22 at most, and 0 where the divisor passes 2^126)
+__device__ __forceinline__ float gated(float o, float gate) { return __fdividef(o, 1.f + __expf(-gate)); }
+// Four dims of a result: weighted values times 1 / sum, times the gate's sigmoid, in bf16.
+__device__ __forceinline__ uint2 finish4(float4 y, float inv, bool has_gate, uint2 gate) {
+    y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
+    if (has_gate) {
+        y.x = gated(y.x, __uint_as_float(gate.x << 16)), y.y = gated(y.y, __uint_as_float(gate.x & 0xffff0000u));
+        y.z = gated(y.z, __uint_as_float(gate.y << 16)), y.w = gated(y.w, __uint_as_float(gate.y & 0xffff0000u));
+    }
+    return make_uint2(pack2(y.x, y.y), pack2(y.z, y.w));
+}
 
 template <int DH, int HB>
 __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
@@ -402,6 +424,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
         const int mine = warp % HB, sub = warp / HB;        // this warp's head of the block, its slice of the tile
         float* sums = reinterpret_cast<float*>(smem + G::OFF_SUM);
         float2* ml = reinterpret_cast<float2*>(smem + G::OFF_ML);
+        float* inverse = reinterpret_cast<float*>(smem + G::OFF_INV);
         const int ra = lane >> 2, rb = ra + 8;              // the two rows (query heads) of this lane's accumulators
         // lane parts of the ldmatrix addresses in the box's tile of 64 dims
         const int k_tok = (lane >> 4) * 8 + (lane & 7), k_ch = (lane >> 3) & 1;
@@ -505,85 +528,93 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
             }
 
             // ---- the piece's end ----
+            // The warps hand their weighted values over in shared memory, some dims at a time, and those of a head
+            // sum, norm and write them. One loop for it, the accumulators moving up: unrolled, the code took longer to
+            // fetch than to run, and every gate waited for the store before it (5 us a piece at 128 dims, 17 at 256).
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) {
                 la += __shfl_xor_sync(0xffffffffu, la, o);
                 lb += __shfl_xor_sync(0xffffffffu, lb, o);
             }
-            if constexpr (SUBS > 1) {
-                // one maximum for the warps of a head, then their sums and weighted values in turn
-                if ((lane & 3) == 0) ml[warp * 16 + ra] = make_float2(ma, la), ml[warp * 16 + rb] = make_float2(mb, lb);
-                consumer_sync();
-                float na = -INFINITY, nb = -INFINITY;
+            if ((lane & 3) == 0) ml[warp * 16 + ra] = make_float2(ma, la), ml[warp * 16 + rb] = make_float2(mb, lb);
+            piece_sync<SUBS>();
+            auto joined = [&](int row) {  // maximum and sum of a row over the warps of the head
+                float m = -INFINITY, l = 0.f;
 #pragma unroll
-                for (int u = 0; u < SUBS; u++) na = fmaxf(na, ml[(u * HB + mine) * 16 + ra].x), nb = fmaxf(nb, ml[(u * HB + mine) * 16 + rb].x);
-                const float oa = na == -INFINITY ? 0.f : na, ob = nb == -INFINITY ? 0.f : nb;
-                const float fa = exp2f(ma - oa), fb = exp2f(mb - ob);
-                la = lb = 0.f;
+                for (int u = 0; u < SUBS; u++) m = fmaxf(m, ml[(u * HB + mine) * 16 + row].x);
 #pragma unroll
                 for (int u = 0; u < SUBS; u++) {
-                    const float2 x = ml[(u * HB + mine) * 16 + ra], y = ml[(u * HB + mine) * 16 + rb];
-                    la += x.y * exp2f(x.x - oa), lb += y.y * exp2f(y.x - ob);
+                    const float2 x = ml[(u * HB + mine) * 16 + row];
+                    l += x.y * exp2f(x.x - (m == -INFINITY ? 0.f : m));
                 }
-                ma = na, mb = nb;
-#pragma unroll
-                for (int t = 0; t < NT; t++) acc[t][0] *= fa, acc[t][1] *= fa, acc[t][2] *= fb, acc[t][3] *= fb;
-#pragma unroll
-                for (int u = 1; u < SUBS; u++)
-#pragma unroll
-                    for (int c = 0; c < NT; c += 8) {
-                        float2* box = reinterpret_cast<float2*>(sums + mine * 16 * 64);
-#pragma unroll
-                        for (int t = 0; t < 8; t++)
-                            if (sub == u) {
-                                box[(t * 2) * 32 + lane] = make_float2(acc[c + t][0], acc[c + t][1]);
-                                box[(t * 2 + 1) * 32 + lane] = make_float2(acc[c + t][2], acc[c + t][3]);
-                            }
-                        consumer_sync();
-#pragma unroll
-                        for (int t = 0; t < 8; t++)
-                            if (sub == 0) {
-                                const float2 x = box[(t * 2) * 32 + lane], y = box[(t * 2 + 1) * 32 + lane];
-                                acc[c + t][0] += x.x, acc[c + t][1] += x.y, acc[c + t][2] += y.x, acc[c + t][3] += y.y;
-                            }
-                        consumer_sync();
-                    }
+                return make_float2(m, l);
+            };
+            float fa = 1.f, fb = 1.f;
+            if constexpr (SUBS > 1) {
+                const float na = joined(ra).x, nb = joined(rb).x;
+                fa = exp2f(ma - (na == -INFINITY ? 0.f : na)), fb = exp2f(mb - (nb == -INFINITY ? 0.f : nb));
             }
             const bool whole = from == 0 && end == w.tiles;
-            if (sub == 0 && whole) {
-                const float ia = la == 0.f ? 0.f : 1.f / la, ib = lb == 0.f ? 0.f : 1.f / lb;
+            // the part that begins a (row, unit) lies in place 1, one that continues it in place 0
+            float* const part_at = a.work + ((size_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * part_floats(HB * a.chunk, DH);
+            if (whole && sub == 0 && lane < heads) {
+                const float l = joined(lane).y;
+                inverse[mine * 16 + lane] = l == 0.f ? 0.f : 1.f / l;
+            }
+            if (!whole && sub == 0 && lane < heads)
+                reinterpret_cast<float2*>(part_at + (size_t)HB * a.chunk * DH)[mine * a.chunk + lane] = joined(lane);
+            if (SUBS == 1 && !whole) {  // nothing to sum or to gate
+                float* val = part_at + (size_t)mine * a.chunk * DH + (lane & 3) * 2;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    const size_t at = q_row + t * 8 + (lane & 3) * 2;
+                    if (ra < heads) *reinterpret_cast<float2*>(val + ra * DH + t * 8) = make_float2(acc[t][0], acc[t][1]);
+                    if (rb < heads) *reinterpret_cast<float2*>(val + rb * DH + t * 8) = make_float2(acc[t][2], acc[t][3]);
+                }
+            }
+            constexpr int QUADS = G::PART / 4, STEPS = 16 * QUADS / (32 * SUBS);  // fours of dims, and how many of them a lane writes
+            float* const box = sums + warp * 16 * G::PITCH;
+            uint2 gate[STEPS];
+            auto gates = [&](int d0) {
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int row = e ? rb : ra;
-                        if (row >= heads) continue;
-                        float y0 = acc[t][2 * e] * (e ? ib : ia), y1 = acc[t][2 * e + 1] * (e ? ib : ia);
-                        if (a.gate) {
-                            const uint32_t g2 = *reinterpret_cast<const uint32_t*>(a.gate + at + (size_t)row * DH);
-                            y0 = gated(y0, __uint_as_float(g2 << 16));
-                            y1 = gated(y1, __uint_as_float(g2 & 0xffff0000u));
-                        }
-                        *reinterpret_cast<uint32_t*>(a.out + at + (size_t)row * DH) = pack2(y0, y1);
+                for (int i = 0; i < STEPS; i++) {
+                    const int at = (i * SUBS + sub) * 32 + lane, row = at / QUADS;
+                    if (a.gate && whole && row < heads)
+                        gate[i] = __ldg(reinterpret_cast<const uint2*>(a.gate + q_row + (size_t)row * DH + d0 + at % QUADS * 4));
+                }
+            };
+            gates(0);
+#pragma unroll 1
+            for (int d0 = SUBS == 1 && !whole ? DH : 0; d0 < DH; d0 += G::PART) {
+#pragma unroll
+                for (int t = 0; t < G::PART / 8; t++) {
+                    const int d = t * 8 + (lane & 3) * 2;
+                    *reinterpret_cast<float2*>(box + ra * G::PITCH + d) = make_float2(acc[t][0] * fa, acc[t][1] * fa);
+                    *reinterpret_cast<float2*>(box + rb * G::PITCH + d) = make_float2(acc[t][2] * fb, acc[t][3] * fb);
+                }
+                piece_sync<SUBS>();
+#pragma unroll
+                for (int i = 0; i < STEPS; i++) {
+                    const int at = (i * SUBS + sub) * 32 + lane, row = at / QUADS, d = at % QUADS * 4;
+                    if (row >= heads) continue;
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int u = 0; u < SUBS; u++) {
+                        const float4 x = *reinterpret_cast<const float4*>(sums + ((u * HB + mine) * 16 + row) * G::PITCH + d);
+                        y.x += x.x, y.y += x.y, y.z += x.z, y.w += x.w;
+                    }
+                    if (whole) {
+                        *reinterpret_cast<uint2*>(a.out + q_row + (size_t)row * DH + d0 + d) =
+                            finish4(y, inverse[mine * 16 + row], a.gate != nullptr, gate[i]);
+                    } else {
+                        *reinterpret_cast<float4*>(part_at + ((size_t)mine * a.chunk + row) * DH + d0 + d) = y;
                     }
                 }
-            } else if (sub == 0) {
-                // the part that begins a (row, unit) lies in place 1, one that continues it in place 0
-                const int place = from == 0 ? 1 : 0;
-                float* dst = a.work + ((size_t)blockIdx.x * 2 + place) * part_floats(HB * a.chunk, DH);
-                float* val = dst + (size_t)mine * a.chunk * DH;
+                if (d0 + G::PART < DH) gates(d0 + G::PART);
+                piece_sync<SUBS>();
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const int d = t * 8 + (lane & 3) * 2;
-                    if (ra < heads) *reinterpret_cast<float2*>(val + ra * DH + d) = make_float2(acc[t][0], acc[t][1]);
-                    if (rb < heads) *reinterpret_cast<float2*>(val + rb * DH + d) = make_float2(acc[t][2], acc[t][3]);
-                }
-                float2* pair = reinterpret_cast<float2*>(dst + (size_t)HB * a.chunk * DH) + mine * a.chunk;
-                if ((lane & 3) == 0) {
-                    if (ra < heads) pair[ra] = make_float2(ma, la);
-                    if (rb < heads) pair[rb] = make_float2(mb, lb);
-                }
+                for (int t = 0; t < NT - G::PART / 8; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[t][e] = acc[t + G::PART / 8][e];
             }
             if (w.left > 0) walk_next_piece<TILE>(a, w);
         }
@@ -703,13 +734,8 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_paged_join_kernel(const 
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const size_t d = at + e * 128 + lane * 4;
-            float y[4] = {acc[e].x * inv, acc[e].y * inv, acc[e].z * inv, acc[e].w * inv};
-            if (a.gate) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) y[k] = gated(y[k], f32(a.gate[d + k]));
-            }
-            *reinterpret_cast<uint32_t*>(a.out + d) = pack2(y[0], y[1]);
-            *reinterpret_cast<uint32_t*>(a.out + d + 2) = pack2(y[2], y[3]);
+            const uint2 gate = a.gate ? __ldg(reinterpret_cast<const uint2*>(a.gate + d)) : make_uint2(0, 0);
+            *reinterpret_cast<uint2*>(a.out + d) = finish4(acc[e], inv, a.gate != nullptr, gate);
         }
     }
 }
@@ -817,8 +843,7 @@ extern "C" int s1_attention_paged(const void* q, const void* gate, void* out, co
     if (rows == 0) return cudaSuccess;
     const PageTable t{table, table_pages, n_seqs, n_pages, page_tokens};
     if (!table_ok(t) || !q || !out || !k_pages || !v_pages || !len || !workspace) return cudaErrorInvalidValue;
-    if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(q) & 3) ||
-        (reinterpret_cast<uintptr_t>(out) & 3) || (reinterpret_cast<uintptr_t>(gate) & 3))
+    if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(workspace) || !aligned16(q) || !aligned16(out) || !aligned16(gate))
         return cudaErrorInvalidValue;
     if (workspace_floats < s1_attention_paged_workspace_floats(Hq, Hk, Dh)) return cudaErrorInvalidValue;
     PagedArgs a{};

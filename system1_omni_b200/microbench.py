@@ -1,6 +1,6 @@
 """Per-operator device timings through the C ABI, against each operator's roofline.
 
-    python -m system1_omni_b200.microbench --what elementwise|gemm|gdn|attention|all [--out file.jsonl]
+    python -m system1_omni_b200.microbench --what elementwise|gemm|gdn|attention|step|all [--out file.jsonl]
 
 elementwise  the elementwise / reduction sweep: bf16 N(0,1)-like activations with
              tokens in {1k, 4k, 16k, 64k} x channels in {2048, 4096, 8192} for causal
@@ -11,6 +11,9 @@ gemm         the projection shapes of the 4B-, 9B- and 27B-shaped decoders at 10
 gdn          the chunked gated delta rule (both kernels of cs1_gdn_prefill) at the reference's
              published shapes (H=48, HK=16, T in {107, 936, 3399}) and the model shapes; microseconds.
 attention    causal GQA flash attention at head dims 128 and 256.
+step         the operators of the tokens after a prefill at the 27B shape (16 qk / 48 v delta-rule heads, 24 q / 4 kv
+             attention heads of 128), one token for each of 1 to 128 sequences, caches of 1000 to 32000 tokens in
+             pages of 64; and the copies of a fork. GB/s = bytes that have to move / device time.
 
 Calls rotate over enough copies of their buffers to exceed the 126 MB L2, so a timing is
 not flattered by a warm cache; every figure is the mean of `--iters` launches between two
@@ -72,6 +75,83 @@ class Bench:
         self.stream.sync()
         L.check(code, "timed call")
         return self.e0.elapsed_ms(self.e1) * 1e3 / self.iters
+
+
+def step(b, out):
+    """One token per sequence through the decode operators."""
+    lib, st = b.lib, b.stream.handle
+    hbm, _, src = peaks()
+    H, HK, Hq, Hk, Dh, half, page = 48, 16, 24, 4, 128, 32, 64
+    kd, vd = HK * 128, H * 128
+    ch = 2 * kd + vd
+    i32 = lambda a: L.to_device(np.asarray(a, np.int32), b.stream)
+
+    def zeros(n):  # what states and caches hold does not change the times
+        buf = L.DeviceBuffer(n)
+        L.check(lib.s1_memset_async(buf.at(), 0, n, st), "memset")
+        return buf
+
+    def report(op, n, tokens, nbytes, us):
+        gbs = nbytes / us * 1e-3
+        out({"bench": "step", "op": op, "sequences": n, "cache_tokens": tokens, "us": round(us, 2), "gb_s": round(gbs, 1),
+             "fraction": round(gbs / hbm, 3), "peak": src})
+
+    for n in (1, 8, 32, 128):
+        slots, state = i32(np.arange(n)), H * 128 * 128 * 4
+        nbytes = n * (2 * state + (2 * kd + 2 * vd + H) * 2 + 4 * H)
+        copies = b.copies(nbytes)
+        rows = [(b.bf16(n * kd), b.bf16(n * kd), b.bf16(n * vd), L.to_device(np.full(n * H, -0.5, np.float32), b.stream), b.bf16(n * H, 0.2),
+                 L.DeviceBuffer(n * vd * 2), zeros(n * state)) for _ in range(copies)]
+        us = b.time(lambda i: lib.s1_gdn_step(*(x.at() for x in rows[i][:6]), n, H, HK, 128 ** -0.5, rows[i][6].at(), n, state // 4, None,
+                                              slots.at(), slots.at(), n, st), copies)
+        report("gdn_step", n, None, nbytes, us)
+        del rows
+
+        ld = ch + vd + 2 * H
+        nbytes = n * (4 * ch + 12 * ch + 10 * H) + 8 * ch
+        copies = b.copies(nbytes)
+        w, al, dt = b.bf16(ch * 4, 0.3), b.bf16(H), b.bf16(H, 0.1)
+        rows = [(b.bf16(n * ld), L.DeviceBuffer(n * kd * 2), L.DeviceBuffer(n * kd * 2), L.DeviceBuffer(n * vd * 2), L.DeviceBuffer(n * H * 2),
+                 L.DeviceBuffer(n * H * 4), b.bf16(n * 3 * ch)) for _ in range(copies)]
+        us = b.time(lambda i: lib.s1_gdn_conv_gates_step(
+            rows[i][0].at(), ld, w.at(), rows[i][1].at(), rows[i][2].at(), rows[i][3].at(), n, kd, vd, rows[i][0].at(2 * (ch + vd)),
+            rows[i][0].at(2 * (ch + vd + H)), al.at(), dt.at(), rows[i][4].at(), rows[i][5].at(), H, rows[i][6].at(), n, 3 * ch, None, slots.at(),
+            slots.at(), n, st), copies)
+        report("gdn_conv_gates_step", n, None, nbytes, us)
+        del rows
+
+        for tokens in (1000, 8000, 32000):
+            if n * tokens > 1 << 20:
+                continue
+            per = -(-tokens // page)
+            table = i32(np.random.default_rng(0).permutation(n * per).reshape(n, per))
+            pos, length = i32(np.full(n, tokens - 1)), i32(np.full(n, tokens))
+            token = Hk * Dh * 2
+            copies = b.copies(2 * n * tokens * token)
+            pools = [(zeros(n * per * page * token), zeros(n * per * page * token)) for _ in range(copies)]
+            q, gate, o = b.bf16(n * Hq * Dh), b.bf16(n * Hq * Dh), L.DeviceBuffer(n * Hq * Dh * 2)
+            ld = 2 * (Hq + Hk) * Dh
+            x, qw, cos = b.bf16(n * ld), b.bf16(Dh, 0.1), b.bf16(tokens * half)
+            us = b.time(lambda i: lib.s1_attn_prep_paged(
+                x.at(), x.at(4 * Hq * Dh), x.at(4 * Hq * Dh + 2 * Hk * Dh), ld, qw.at(), qw.at(), cos.at(), cos.at(), tokens, None, q.at(), gate.at(),
+                pools[i][0].at(), pools[i][1].at(), n * per, page, table.at(), per, n, None, pos.at(), n, Hq, Hk, Dh, half, 1e-6, st), copies)
+            report("attn_prep_paged", n, tokens, n * (2 * ld * 2 + 4 * half), us)
+            floats = lib.s1_attention_paged_workspace_floats(Hq, Hk, Dh)
+            ws = L.DeviceBuffer(floats * 4)
+            us = b.time(lambda i: lib.s1_attention_paged(
+                q.at(), gate.at(), o.at(), pools[i][0].at(), pools[i][1].at(), n * per, page, table.at(), per, n, None, length.at(), n, Hq, Hk, Dh,
+                Dh ** -0.5, ws.at(), floats, st), copies)
+            report("attention_paged", n, tokens, 2 * n * tokens * token + 6 * n * Hq * Dh, us)
+            del pools
+
+    # the state and a page of keys and values of every layer (48 delta-rule, 16 attention) for 8 candidates of a prefix
+    for op, layers, nbytes in (("fork_states", 48, H * 128 * 128 * 4), ("fork_pages", 32, page * Hk * Dh * 2)):
+        pools = [L.DeviceBuffer(9 * nbytes) for _ in range(layers)]
+        ptrs = (C.c_void_p * layers)(*[p.ptr.value for p in pools])
+        a, d = np.zeros(8, np.int32), np.arange(1, 9, dtype=np.int32)
+        us = b.time(lambda i: lib.s1_pages_copy(ptrs, layers, 9, nbytes, a.ctypes.data, d.ctypes.data, 8, st), 1)
+        report(op, 8, None, 9 * layers * nbytes, us)
+        del pools
 
 
 def elementwise(b, out):
@@ -532,7 +612,7 @@ def attention(b, out):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--what", default="all", choices=["elementwise", "gemm", "gdn", "layer", "attention", "prefix", "candidates", "requests", "single", "latency", "all"])
+    ap.add_argument("--what", default="all", choices=["elementwise", "gemm", "gdn", "layer", "attention", "step", "prefix", "candidates", "requests", "single", "latency", "all"])
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--iters", type=int, default=30)
     ap.add_argument("--out", default=None)
@@ -564,7 +644,7 @@ def main():
             sink.write(line + "\n")
 
     for name, fn in (("elementwise", elementwise), ("gemm", gemm), ("gdn", gdn), ("layer", layer),
-                     ("attention", attention)):
+                     ("attention", attention), ("step", step)):
         if args.what in (name, "all"):
             fn(b, out)
     if args.what == "prefix":  # builds a 9B-shaped model (14 GB of weights): only on request

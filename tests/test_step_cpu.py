@@ -260,8 +260,8 @@ def attention(cs1, **kw):
 
 @pytest.mark.parametrize("bad", [dict(Dh=64), dict(Hk=3), dict(Hk=0), dict(Hq=0), dict(rows=-1), dict(rows=(1 << 20) + 1), dict(page=8),
                                  dict(page=24), dict(page=0), dict(n_pages=0), dict(n_pages=1 << 27), dict(wide=0), dict(wide=1 << 27),
-                                 dict(seqs=0), dict(table=None), dict(len=None), dict(q=None), dict(q=A + 2), dict(out=None),
-                                 dict(out=A + 2), dict(gate=A + 2), dict(kp=None), dict(kp=A + 8), dict(vp=A + 2), dict(ws=None),
+                                 dict(seqs=0), dict(table=None), dict(len=None), dict(q=None), dict(q=A + 8), dict(out=None),
+                                 dict(out=A + 4), dict(gate=A + 2), dict(kp=None), dict(kp=A + 8), dict(vp=A + 2), dict(ws=None),
                                  dict(ws=A + 4), dict(floats=100)])
 def test_paged_attention_refuses(cs1, bad):
     assert attention(cs1, **bad) == INVALID
