@@ -536,13 +536,23 @@ def test_paged_attention_matches_the_formula(cs1, stream, Dh, Hq, Hk, page, gate
 @pytest.mark.parametrize("Dh,Hq,Hk,page,lens", [
     (128, 24, 4, 64, [20001]), (256, 16, 4, 16, [9001]), (128, 4, 1, 16, [40000, 3, 5000]), (256, 8, 8, 80, [1, 6000, 64]),
     (128, 16, 4, 32, [1]), (128, 16, 4, 32, [0]), (128, 16, 4, 32, [-1, -1]), (128, 6, 2, 16, [64] * 200), (256, 6, 1, 256, [513] * 75),
-    (128, 24, 4, 64, [500 + 37 * i for i in range(60)])])
+    (128, 24, 4, 64, [500 + 37 * i for i in range(60)]), (128, 9, 3, 1024, [5000, 1024, 1025]), (256, 64, 1, 16, [700, 33]),
+    (256, 12, 6, 4096, [4096, 1, 9000])])
 def test_paged_attention_cut_over_many_blocks(cs1, stream, Dh, Hq, Hk, page, lens):
     """Rows cut in the middle, at their ends, into one tile each; many rows per block; nothing at all."""
     c = attn_case(lens, Hq, Hk, Dh, page, len(lens) + Dh)
     got = run_attn(cs1, stream, c, True, Dh ** -0.5)
     rows = range(len(lens)) if len(lens) < 20 else range(0, len(lens), 7)
     check_attn(c, got, True, Dh ** -0.5, rows)
+
+
+def test_paged_attention_of_very_many_rows(cs1, stream):
+    """More rows than a block has threads, most of them next to nothing: lengths 0, 1, 17, 40 and rows that sit out."""
+    lens = [(0, 1, -1, 17, 1, 40, 0)[(i * i) % 7] for i in range(20011)]
+    seq = [i % 50 for i in range(len(lens))]
+    c = attn_case(lens, 2, 1, 128, 16, 9, seq=seq)
+    got = run_attn(cs1, stream, c, True, 128 ** -0.5)
+    check_attn(c, got, True, 128 ** -0.5, list(range(0, len(lens), 97)) + list(range(len(lens) - 20, len(lens))))
 
 
 def test_paged_attention_rows_of_one_sequence_are_a_causal_window(cs1, stream):
@@ -686,6 +696,26 @@ def test_page_copies(cs1, stream, page_bytes, n_pools, n_pages, pairs, fan):
         want = p.copy()
         want[order[n_pages - pairs:]] = p[order[:pairs][np.arange(pairs) // fan]]
         assert (down(b, p.shape, stream, np.uint8) == want).all()
+
+
+def test_recorded_page_copies_keep_their_lists(cs1, stream):
+    st = L.Stream()
+    pool = np.arange(6 * 16, dtype=np.uint8).reshape(6, 16)
+    buf = up(pool, st)
+    ptrs = (C.c_void_p * 1)(buf.ptr.value)
+    src, dst = np.array([0, 0, 1], np.int32), np.array([3, 4, 5], np.int32)
+    exec_ = C.c_void_p()
+    L.check(cs1.cs1_graph_begin(st.handle), "begin")
+    L.check(cs1.s1_pages_copy(ptrs, 1, 6, 16, src.ctypes.data, dst.ctypes.data, 3, st.handle), "copy")
+    L.check(cs1.cs1_graph_end(st.handle, C.byref(exec_)), "end")
+    src[:], dst[:], ptrs[0] = 2, 2, None
+    for k in range(2):
+        pool[:2] += 7
+        L.check(cs1.cs1_upload(buf.at(), pool.ctypes.data, pool.nbytes, st.handle), "upload")
+        L.check(cs1.cs1_graph_launch(exec_, st.handle), "launch")
+        pool[[3, 4, 5]] = pool[[0, 0, 1]]
+        assert (down(buf, pool.shape, st, np.uint8) == pool).all()
+    cs1.cs1_graph_destroy(exec_)
 
 
 # ---- together ----
