@@ -215,8 +215,9 @@ __device__ __forceinline__ long long row_tiles(const PagedArgs& a, int r, int& t
 
 // The cut of a line of `total` tiles into runs, one per block, none of them empty but those behind the last.
 // (SMs do not stream equally fast: the first block ends some 15 % before the last. Equal runs over three
-// quarters and a finer cut of the rest, for the blocks that end first, was slower all the same, 103.7 -> 107 us
-// at 307,000 tokens of 4 heads: a block's start costs more than it evens out.)
+// quarters and a finer cut of the rest, for whoever is done first, was slower all the same: at 307,000 tokens of 4
+// heads 104 -> 107 us as blocks that follow, 118 as blocks that the resident ones take over. A run's start and
+// its part cost more than they even out.)
 struct Cut {
     long long total;
     int runs;
