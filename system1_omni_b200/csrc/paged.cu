@@ -537,6 +537,22 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                 la += __shfl_xor_sync(0xffffffffu, la, o);
                 lb += __shfl_xor_sync(0xffffffffu, lb, o);
             }
+            const bool whole = from == 0 && end == w.tiles;
+            // the part that begins a (row, unit) lies in place 1, one that continues it in place 0
+            float* const part_at = a.work + ((size_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * part_floats(HB * a.chunk, DH);
+            float2* const pairs_at = reinterpret_cast<float2*>(part_at + (size_t)HB * a.chunk * DH) + mine * a.chunk;
+            if (SUBS == 1 && !whole) {  // nothing to sum or to gate
+                float* val = part_at + (size_t)mine * a.chunk * DH + (lane & 3) * 2;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    if (ra < heads) *reinterpret_cast<float2*>(val + ra * DH + t * 8) = make_float2(acc[t][0], acc[t][1]);
+                    if (rb < heads) *reinterpret_cast<float2*>(val + rb * DH + t * 8) = make_float2(acc[t][2], acc[t][3]);
+                }
+                if ((lane & 3) == 0 && ra < heads) pairs_at[ra] = make_float2(ma, la);
+                if ((lane & 3) == 0 && rb < heads) pairs_at[rb] = make_float2(mb, lb);
+                if (w.left > 0) walk_next_piece<TILE>(a, w);
+                continue;
+            }
             if ((lane & 3) == 0) ml[warp * 16 + ra] = make_float2(ma, la), ml[warp * 16 + rb] = make_float2(mb, lb);
             piece_sync<SUBS>();
             auto joined = [&](int row) {  // maximum and sum of a row over the warps of the head
@@ -555,22 +571,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                 const float na = joined(ra).x, nb = joined(rb).x;
                 fa = exp2f(ma - (na == -INFINITY ? 0.f : na)), fb = exp2f(mb - (nb == -INFINITY ? 0.f : nb));
             }
-            const bool whole = from == 0 && end == w.tiles;
-            // the part that begins a (row, unit) lies in place 1, one that continues it in place 0
-            float* const part_at = a.work + ((size_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * part_floats(HB * a.chunk, DH);
-            if (whole && sub == 0 && lane < heads) {
-                const float l = joined(lane).y;
-                inverse[mine * 16 + lane] = l == 0.f ? 0.f : 1.f / l;
-            }
-            if (!whole && sub == 0 && lane < heads)
-                reinterpret_cast<float2*>(part_at + (size_t)HB * a.chunk * DH)[mine * a.chunk + lane] = joined(lane);
-            if (SUBS == 1 && !whole) {  // nothing to sum or to gate
-                float* val = part_at + (size_t)mine * a.chunk * DH + (lane & 3) * 2;
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    if (ra < heads) *reinterpret_cast<float2*>(val + ra * DH + t * 8) = make_float2(acc[t][0], acc[t][1]);
-                    if (rb < heads) *reinterpret_cast<float2*>(val + rb * DH + t * 8) = make_float2(acc[t][2], acc[t][3]);
-                }
+            if (sub == 0 && lane < heads) {
+                const float2 x = joined(lane);
+                if (whole)
+                    inverse[mine * 16 + lane] = x.y == 0.f ? 0.f : 1.f / x.y;
+                else
+                    pairs_at[lane] = x;
             }
             constexpr int QUADS = G::PART / 4, STEPS = 16 * QUADS / (32 * SUBS);  // fours of dims, and how many of them a lane writes
             float* const box = sums + warp * 16 * G::PITCH;
@@ -585,7 +591,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
             };
             gates(0);
 #pragma unroll 1
-            for (int d0 = SUBS == 1 && !whole ? DH : 0; d0 < DH; d0 += G::PART) {
+            for (int d0 = 0; d0 < DH; d0 += G::PART) {
 #pragma unroll
                 for (int t = 0; t < G::PART / 8; t++) {
                     const int d = t * 8 + (lane & 3) * 2;
@@ -675,6 +681,11 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_paged_join_kernel(const 
         const size_t at = ((size_t)note.x * a.Hq + (size_t)hk * a.group + h0 + i) * DH;
         float m = -INFINITY, l = 0.f;
         float4 acc[E] = {};
+        uint2 gate[E] = {};
+        if (a.gate && (!together || warp == 0)) {
+#pragma unroll
+            for (int e = 0; e < E; e++) gate[e] = __ldg(reinterpret_cast<const uint2*>(a.gate + at + e * 128 + lane * 4));
+        }
         const int stride = together ? JOIN_WARPS : 1;
         for (int p0 = b + (together ? warp : 0); p0 <= note.z; p0 += U * stride) {
             float2 ml[U];
@@ -735,8 +746,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_paged_join_kernel(const 
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const size_t d = at + e * 128 + lane * 4;
-            const uint2 gate = a.gate ? __ldg(reinterpret_cast<const uint2*>(a.gate + d)) : make_uint2(0, 0);
-            *reinterpret_cast<uint2*>(a.out + d) = finish4(acc[e], inv, a.gate != nullptr, gate);
+            *reinterpret_cast<uint2*>(a.out + d) = finish4(acc[e], inv, a.gate != nullptr, gate[e]);
         }
     }
 }
