@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __g
 // first kernel alone takes 100 us of it: what is left is its start (2.4 us to the first tile) and the join.
 constexpr int CONSUMERS = 4, PAGED_THREADS = (CONSUMERS + 1) * 32;
 constexpr int SLICE = 16;       // tokens of a warp's part of a tile, and of a copied box
-constexpr int MIN_RUN = 1;      // tiles
+constexpr int RUN = 8, PARTS = 96;  // tiles of a run, parts of a piece: see Cut
 constexpr int MAX_GROUP = 16;   // query heads of one key-value head that a block takes at once
 constexpr int MAX_BLOCKS = 296; // two per SM
 
@@ -214,6 +214,10 @@ __device__ __forceinline__ long long row_tiles(const PagedArgs& a, int r, int& t
 }
 
 // The cut of a line of `total` tiles into runs, one per block, none of them empty but those behind the last.
+// Runs of one tile as long as the pieces ((row, head block)s, `pieces` of them) come to PARTS parts each on
+// average, which the join takes in one trip (16 warps with 6 in flight); from there on runs grow to RUN tiles
+// before more parts are made. One row of 24 and 4 heads of 128, a run per block at all lengths and this: 1500
+// tokens 9.0 and 9.1 us, 5000: 13.7 and 11.4, 8000: 15.3 and 12.9, 24000: 20.9 and 18.6, from 38000 on the same.
 // (SMs do not stream equally fast: the first block ends some 15 % before the last. Equal runs over three
 // quarters and a finer cut of the rest, for whoever is done first, was slower all the same: at 307,000 tokens of 4
 // heads 104 -> 107 us as blocks that follow, 118 as blocks that the resident ones take over. A run's start and
@@ -222,7 +226,8 @@ struct Cut {
     long long total;
     int runs;
     Cut() = default;
-    __device__ Cut(long long t, int blocks) : total(t), runs((int)min((long long)blocks, (t + MIN_RUN - 1) / MIN_RUN)) {}
+    __device__ Cut(long long t, int blocks, long long pieces)
+        : total(t), runs((int)min((long long)blocks, min(t, max((t + RUN - 1) / RUN, PARTS * pieces)))) {}
     __device__ long long begin(int r) const { return r >= runs ? total : total * r / runs; }
     // The last run that begins at or before tile t: floor(total r / runs) <= t just where r <= (runs (t + 1) - 1) / total.
     __device__ int run_of(long long t) const { return (int)((runs * (t + 1) - 1) / total); }
@@ -336,7 +341,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
             if (w < warp) upto += warp_sums[w];
             total += warp_sums[w];
         }
-        const Cut cut(total, gridDim.x);
+        const Cut cut(total, gridDim.x, (long long)a.rows * a.units);
         const long long lo = cut.begin(blockIdx.x), hi = cut.begin(blockIdx.x + 1);
         if (tid == 0) whole_cut = cut;
         if (tid == 0 && lo == hi) begin.left = 0;
@@ -431,21 +436,28 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
         const int k_tok = (lane >> 4) * 8 + (lane & 7), k_ch = (lane >> 3) & 1;
         const int v_tok = lane & 15, v_ch = lane >> 4;
         const uint32_t my_tiles = sub * BOX_BYTES + mine * (DH / 64) * (SLICE * 128);
+        // where in q, gate and out the heads of a piece begin, and how many they are
+        auto place = [&](int unit, int row, int& heads) {
+            const int h0 = unit % a.chunks * a.chunk;
+            heads = min(a.chunk, a.group - h0);
+            return ((size_t)row * a.Hq + (size_t)(unit / a.chunks * HB + mine) * a.group + h0) * DH;
+        };
         uint32_t it = 0;
         bool ok = true;
         while (w.left > 0) {
             const int n = a.len[w.row];
-            const int hk = w.unit / a.chunks * HB + mine, part = w.unit % a.chunks;
-            const int h0 = part * a.chunk, heads = min(a.chunk, a.group - h0);
-            const size_t q_row = ((size_t)w.row * a.Hq + (size_t)hk * a.group + h0) * DH;
             uint32_t qf[DH / 16][4];
+            {
+                int heads;
+                const size_t q_row = place(w.unit, w.row, heads);
 #pragma unroll
-            for (int ks = 0; ks < DH / 16; ks++) {
-                const bf16* src = a.q + q_row + ks * 16 + (lane & 3) * 2;
-                qf[ks][0] = ra < heads ? *reinterpret_cast<const uint32_t*>(src + (size_t)ra * DH) : 0;
-                qf[ks][1] = rb < heads ? *reinterpret_cast<const uint32_t*>(src + (size_t)rb * DH) : 0;
-                qf[ks][2] = ra < heads ? *reinterpret_cast<const uint32_t*>(src + (size_t)ra * DH + 8) : 0;
-                qf[ks][3] = rb < heads ? *reinterpret_cast<const uint32_t*>(src + (size_t)rb * DH + 8) : 0;
+                for (int ks = 0; ks < DH / 16; ks++) {
+                    const bf16* src = a.q + q_row + ks * 16 + (lane & 3) * 2;
+                    qf[ks][0] = ra < heads ? *reinterpret_cast<const uint32_t*>(src + (size_t)ra * DH) : 0;
+                    qf[ks][1] = rb < heads ? *reinterpret_cast<const uint32_t*>(src + (size_t)rb * DH) : 0;
+                    qf[ks][2] = ra < heads ? *reinterpret_cast<const uint32_t*>(src + (size_t)ra * DH + 8) : 0;
+                    qf[ks][3] = rb < heads ? *reinterpret_cast<const uint32_t*>(src + (size_t)rb * DH + 8) : 0;
+                }
             }
             float acc[NT][4] = {};
             float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
@@ -537,6 +549,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                 la += __shfl_xor_sync(0xffffffffu, la, o);
                 lb += __shfl_xor_sync(0xffffffffu, lb, o);
             }
+            // Places are computed again from what the compiler takes for new values: held in registers through the
+            // loop they would spill some of its own.
+            int unit = w.unit, heads, own = threadIdx.x;
+            asm volatile("" : "+r"(unit), "+r"(own));
+            const size_t q_row = place(unit, w.row, heads);
+            const int lane = own & 31, warp = own >> 5, mine = warp % HB, sub = warp / HB, ra = lane >> 2, rb = ra + 8;
             const bool whole = from == 0 && end == w.tiles;
             // the part that begins a (row, unit) lies in place 1, one that continues it in place 0
             float* const part_at = a.work + ((size_t)blockIdx.x * 2 + (from == 0 ? 1 : 0)) * part_floats(HB * a.chunk, DH);

@@ -546,6 +546,15 @@ def test_paged_attention_cut_over_many_blocks(cs1, stream, Dh, Hq, Hk, page, len
     check_attn(c, got, True, Dh ** -0.5, rows)
 
 
+@pytest.mark.parametrize("Hq,Hk,tile,tiles", [(Hq, Hk, tile, tiles) for Hq, Hk, tile in ((8, 4, 16), (6, 2, 32), (3, 1, 64))
+                                              for tiles in (95, 96, 97, 191, 767, 768, 769, 2367, 2369) if tiles * tile < 80000])
+def test_paged_attention_where_runs_grow(cs1, stream, Hq, Hk, tile, tiles):
+    """One row at the tile counts where its runs go from one tile to eight, and from there to one per block."""
+    for n in (tiles * tile, tiles * tile - tile + 1):
+        c = attn_case([n], Hq, Hk, 128, 64, tiles + tile)
+        check_attn(c, run_attn(cs1, stream, c, True, 128 ** -0.5), True, 128 ** -0.5)
+
+
 def test_paged_attention_of_very_many_rows(cs1, stream):
     """More rows than a block has threads, most of them next to nothing: lengths 0, 1, 17, 40 and rows that sit out."""
     lens = [(0, 1, -1, 17, 1, 40, 0)[(i * i) % 7] for i in range(20011)]
