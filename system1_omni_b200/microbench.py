@@ -79,7 +79,9 @@ class Bench:
 
 def step(b, out):
     """One token per sequence through the decode operators."""
-    lib, st = b.lib, b.stream.handle
+    lib, st = b.lib, b.stream.handle.value
+    # plain numbers: to convert pointer objects takes longer than some of these run
+    at = lambda buf, offset=0: buf.ptr.value + offset
     hbm, _, src = peaks()
     H, HK, Hq, Hk, Dh, half, page = 48, 16, 24, 4, 128, 32, 64
     kd, vd = HK * 128, H * 128
@@ -88,7 +90,7 @@ def step(b, out):
 
     def zeros(n):  # what states and caches hold does not change the times
         buf = L.DeviceBuffer(n)
-        L.check(lib.s1_memset_async(buf.at(), 0, n, st), "memset")
+        L.check(lib.s1_memset_async(at(buf), 0, n, st), "memset")
         return buf
 
     def report(op, n, tokens, nbytes, us):
@@ -102,8 +104,8 @@ def step(b, out):
         copies = b.copies(nbytes)
         rows = [(b.bf16(n * kd), b.bf16(n * kd), b.bf16(n * vd), L.to_device(np.full(n * H, -0.5, np.float32), b.stream), b.bf16(n * H, 0.2),
                  L.DeviceBuffer(n * vd * 2), zeros(n * state)) for _ in range(copies)]
-        us = b.time(lambda i: lib.s1_gdn_step(*(x.at() for x in rows[i][:6]), n, H, HK, 128 ** -0.5, rows[i][6].at(), n, state // 4, None,
-                                              slots.at(), slots.at(), n, st), copies)
+        us = b.time(lambda i: lib.s1_gdn_step(*(at(x) for x in rows[i][:6]), n, H, HK, 128 ** -0.5, at(rows[i][6]), n, state // 4, None,
+                                              at(slots), at(slots), n, st), copies)
         report("gdn_step", n, None, nbytes, us)
         del rows
 
@@ -114,9 +116,9 @@ def step(b, out):
         rows = [(b.bf16(n * ld), L.DeviceBuffer(n * kd * 2), L.DeviceBuffer(n * kd * 2), L.DeviceBuffer(n * vd * 2), L.DeviceBuffer(n * H * 2),
                  L.DeviceBuffer(n * H * 4), b.bf16(n * 3 * ch)) for _ in range(copies)]
         us = b.time(lambda i: lib.s1_gdn_conv_gates_step(
-            rows[i][0].at(), ld, w.at(), rows[i][1].at(), rows[i][2].at(), rows[i][3].at(), n, kd, vd, rows[i][0].at(2 * (ch + vd)),
-            rows[i][0].at(2 * (ch + vd + H)), al.at(), dt.at(), rows[i][4].at(), rows[i][5].at(), H, rows[i][6].at(), n, 3 * ch, None, slots.at(),
-            slots.at(), n, st), copies)
+            at(rows[i][0]), ld, at(w), at(rows[i][1]), at(rows[i][2]), at(rows[i][3]), n, kd, vd, at(rows[i][0], 2 * (ch + vd)),
+            at(rows[i][0], 2 * (ch + vd + H)), at(al), at(dt), at(rows[i][4]), at(rows[i][5]), H, at(rows[i][6]), n, 3 * ch, None, at(slots),
+            at(slots), n, st), copies)
         report("gdn_conv_gates_step", n, None, nbytes, us)
         del rows
 
@@ -133,14 +135,14 @@ def step(b, out):
             ld = 2 * (Hq + Hk) * Dh
             x, qw, cos = b.bf16(n * ld), b.bf16(Dh, 0.1), b.bf16(tokens * half)
             us = b.time(lambda i: lib.s1_attn_prep_paged(
-                x.at(), x.at(4 * Hq * Dh), x.at(4 * Hq * Dh + 2 * Hk * Dh), ld, qw.at(), qw.at(), cos.at(), cos.at(), tokens, None, q.at(), gate.at(),
-                pools[i][0].at(), pools[i][1].at(), n * per, page, table.at(), per, n, None, pos.at(), n, Hq, Hk, Dh, half, 1e-6, st), copies)
+                at(x), at(x, 4 * Hq * Dh), at(x, 4 * Hq * Dh + 2 * Hk * Dh), ld, at(qw), at(qw), at(cos), at(cos), tokens, None, at(q), at(gate),
+                at(pools[i][0]), at(pools[i][1]), n * per, page, at(table), per, n, None, at(pos), n, Hq, Hk, Dh, half, 1e-6, st), copies)
             report("attn_prep_paged", n, tokens, n * (2 * ld * 2 + 4 * half), us)
             floats = lib.s1_attention_paged_workspace_floats(Hq, Hk, Dh)
             ws = L.DeviceBuffer(floats * 4)
             us = b.time(lambda i: lib.s1_attention_paged(
-                q.at(), gate.at(), o.at(), pools[i][0].at(), pools[i][1].at(), n * per, page, table.at(), per, n, None, length.at(), n, Hq, Hk, Dh,
-                Dh ** -0.5, ws.at(), floats, st), copies)
+                at(q), at(gate), at(o), at(pools[i][0]), at(pools[i][1]), n * per, page, at(table), per, n, None, at(length), n, Hq, Hk, Dh,
+                Dh ** -0.5, at(ws), floats, st), copies)
             report("attention_paged", n, tokens, 2 * n * tokens * token + 6 * n * Hq * Dh, us)
             del pools
 
@@ -149,7 +151,8 @@ def step(b, out):
         pools = [L.DeviceBuffer(9 * nbytes) for _ in range(layers)]
         ptrs = (C.c_void_p * layers)(*[p.ptr.value for p in pools])
         a, d = np.zeros(8, np.int32), np.arange(1, 9, dtype=np.int32)
-        us = b.time(lambda i: lib.s1_pages_copy(ptrs, layers, 9, nbytes, a.ctypes.data, d.ctypes.data, 8, st), 1)
+        src, dst = a.ctypes.data, d.ctypes.data
+        us = b.time(lambda i: lib.s1_pages_copy(C.addressof(ptrs), layers, 9, nbytes, src, dst, 8, st), 1)
         report(op, 8, None, 9 * layers * nbytes, us)
         del pools
 
