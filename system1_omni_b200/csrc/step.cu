@@ -54,10 +54,12 @@ __device__ __forceinline__ void unpack4(uint2 p, float (&x)[4]) {
 // HBM bounds it with one token a sequence: 64 KiB of state in, 64 KiB out per head, all of a block's reads
 // issued at once. Measured at 193 sequences of 48 heads (1.22 GB): 186 us, 6.55 TB/s; columns per warp and
 // blocks per SM at least: 32 and 2: 189 us, 16 and 2: 228, 8 and 2: 276 (narrower warps fetch pieces of lines).
-// Windows are bound by the FMA pipe's latency, a third of its rate, with the three warps per scheduler that such
-// registers leave: 37 windows of 1 to 9 tokens, 32 heads, 38 us (the bytes alone 13). The products of eight
-// tokens at once on the tensor cores with the state split into three bf16 took 39 to 43 us, two resident blocks
-// that prefetch the next state into shared memory 49 to 55.
+// Windows are bound by latency (shared memory first, then the FMAs), with the 2.7 warps per scheduler that such
+// registers leave: 37 windows of 1 to 9 tokens, 32 heads, 38 us (the bytes alone 13), the FMA pipe active for 33 %.
+// The products of eight tokens at once on the tensor cores with the state split into three bf16 took 39 to 43
+// us, two resident blocks that prefetch the next state into shared memory 49 to 55, twice the warps with half the
+// columns 44 to 52, the longest windows first 37.5, and a state kept divided by its decay, a quarter fewer FMAs, 37.5
+// too, with 10.2 for 9.6 us for 3 windows of 9 tokens.
 constexpr int CW = 32, CHUNK = 8, FEW_HEADS = 296;
 
 __device__ __forceinline__ void copy16(const void* dst, const void* src) {
