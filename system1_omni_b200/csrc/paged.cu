@@ -159,13 +159,13 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __g
 // float32 in the workspace, and a second kernel joins the parts of each in order.
 //
 // Measured, in a recorded graph: 65 caches of 500 to 16000 tokens, 24 query and 4 key-value heads of 128
-// (630 MB): 104 us, 6.1 TB/s with the join; 250001 tokens, 16 and 4 heads of 256 (1.02 GB): 159 us, 6.4 TB/s;
-// 1500 tokens: 9.1 us, of which the join is 3.6; 2 tokens: 7. Before, tiles of 64 tokens of one head whose warps
+// (630 MB): 103 us, 6.1 TB/s with the join; 250001 tokens, 16 and 4 heads of 256 (1.02 GB): 158 us, 6.5 TB/s;
+// 1500 tokens: 8.2 us, of which the join is 2.8; 2 tokens: 7. Before, tiles of 64 tokens of one head whose warps
 // shared every tile's maximum and probabilities: 119 us (one block per SM), 113 (two) for the first. The
 // first kernel alone takes 100 us of it: what is left is its start (2.4 us to the first tile) and the join.
 constexpr int CONSUMERS = 4, PAGED_THREADS = (CONSUMERS + 1) * 32;
 constexpr int SLICE = 16;       // tokens of a warp's part of a tile, and of a copied box
-constexpr int RUN = 8, PARTS = 96;  // tiles of a run, parts of a piece: see Cut
+constexpr int RUN = 8, PARTS = 64;  // tiles of a run, parts of a piece: see Cut
 constexpr int MAX_GROUP = 16;   // query heads of one key-value head that a block takes at once
 constexpr int MAX_BLOCKS = 296; // two per SM
 
@@ -200,24 +200,25 @@ struct PagedMaps {
 };
 
 // Workspace: [blocks][2] parts of [heads][DH] weighted values and [heads] (maximum, sum) pairs, in whole
-// 16 bytes (heads = HB * chunk), then int4 [blocks] notes.
+// 16 bytes (heads = HB * chunk).
 __host__ __device__ inline size_t part_floats(int heads, int DH) { return (size_t)heads * DH + (2 * heads + 3) / 4 * 4; }
 
-// Tiles of a row over all its units; 0 for a row that sits out, is empty or is refused.
-template <int TILE>
-__device__ __forceinline__ long long row_tiles(const PagedArgs& a, int r, int& tiles) {
-    const int n = a.len[r], sq = a.seq ? a.seq[r] : r;
+// Tiles of a row over all its units; 0 for a row that sits out, is empty or is refused. PAST_L1: read from L2, for
+// a kernel that runs ahead of the one before it.
+template <bool PAST_L1 = false>
+__device__ __forceinline__ long long row_tiles(const PagedArgs& a, int r, int tile, int& tiles) {
+    const int n = PAST_L1 ? __ldcg(a.len + r) : a.len[r], sq = !a.seq ? r : PAST_L1 ? __ldcg(a.seq + r) : a.seq[r];
     tiles = 0;
     if (n <= 0 || sq < 0 || sq >= a.table.sequences || n > (long long)a.table.width * a.table.page_tokens) return 0;
-    tiles = (n + TILE - 1) / TILE;
+    tiles = (n + tile - 1) / tile;
     return (long long)tiles * a.units;
 }
 
 // The cut of a line of `total` tiles into runs, one per block, none of them empty but those behind the last.
 // Runs of one tile as long as the pieces ((row, head block)s, `pieces` of them) come to PARTS parts each on
-// average, which the join takes in one trip (16 warps with 6 in flight); from there on runs grow to RUN tiles
+// average, which the join takes in one trip (16 warps with 4 in flight); from there on runs grow to RUN tiles
 // before more parts are made. One row of 24 and 4 heads of 128, a run per block at all lengths and this: 1500
-// tokens 9.0 and 9.1 us, 5000: 13.7 and 11.4, 8000: 15.3 and 12.9, 24000: 20.9 and 18.6, from 38000 on the same.
+// tokens 8.2 us both, 5000: 12.9 and 10.7, 8000: 14.6 and 12.7, 24000: 20.2 and 17.7, from 38000 on the same.
 // (SMs do not stream equally fast: the first block ends some 15 % before the last. Equal runs over three
 // quarters and a finer cut of the rest, for whoever is done first, was slower all the same: at 307,000 tokens of 4
 // heads 104 -> 107 us as blocks that follow, 118 as blocks that the resident ones take over. A run's start and
@@ -228,9 +229,13 @@ struct Cut {
     Cut() = default;
     __device__ Cut(long long t, int blocks, long long pieces)
         : total(t), runs((int)min((long long)blocks, min(t, max((t + RUN - 1) / RUN, PARTS * pieces)))) {}
-    __device__ long long begin(int r) const { return r >= runs ? total : total * r / runs; }
+    // (up to 2^22 tiles, 67 million tokens, in 32 bits, whose division is shorter)
+    __device__ bool small() const { return total < 1 << 22; }
+    __device__ long long begin(int r) const { return r >= runs ? total : small() ? (uint32_t)total * r / (uint32_t)runs : total * r / runs; }
     // The last run that begins at or before tile t: floor(total r / runs) <= t just where r <= (runs (t + 1) - 1) / total.
-    __device__ int run_of(long long t) const { return (int)((runs * (t + 1) - 1) / total); }
+    __device__ int run_of(long long t) const {
+        return small() ? (int)(((uint32_t)runs * (uint32_t)(t + 1) - 1) / (uint32_t)total) : (int)((runs * (t + 1) - 1) / total);
+    }
 };
 
 // Position in the line of tiles.
@@ -245,7 +250,7 @@ __device__ __forceinline__ void walk_next_piece(const PagedArgs& a, Walk& w) {
     w.unit = 0;
     do {
         w.row++;
-    } while (w.row < a.rows && row_tiles<TILE>(a, w.row, w.tiles) == 0);
+    } while (w.row < a.rows && row_tiles(a, w.row, TILE, w.tiles) == 0);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -302,10 +307,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
     volatile int* gave_up = reinterpret_cast<volatile int*>(empty + G::STAGES);
     __shared__ long long warp_sums[PAGED_THREADS / 32];
     __shared__ Walk begin;
-    __shared__ Cut whole_cut;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    grid_dep_trigger();
     if (tid == 0) {
         for (int s = 0; s < G::STAGES; s++) {
             mbar_init(&full[s], 1);
@@ -317,6 +320,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
         prefetch_tmap(&maps.v);
     }
     grid_dep_sync();
+    grid_dep_trigger();  // not before: the join reads the lengths without a wait of its own
 
     // ---- this block's run of the line of tiles ----
     {
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
         long long mine = 0;
         for (int r = r0; r < r1; r++) {
             int tiles;
-            mine += row_tiles<TILE>(a, r, tiles);
+            mine += row_tiles(a, r, TILE, tiles);
         }
         long long upto = mine;
 #pragma unroll
@@ -343,13 +347,12 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
         }
         const Cut cut(total, gridDim.x, (long long)a.rows * a.units);
         const long long lo = cut.begin(blockIdx.x), hi = cut.begin(blockIdx.x + 1);
-        if (tid == 0) whole_cut = cut;
         if (tid == 0 && lo == hi) begin.left = 0;
         if (lo < hi && upto - mine <= lo && lo < upto) {
             long long at = upto - mine;
             for (int r = r0; r < r1; r++) {
                 int tiles;
-                const long long n = row_tiles<TILE>(a, r, tiles);
+                const long long n = row_tiles(a, r, TILE, tiles);
                 if (lo < at + n) {
                     const int in_row = (int)(lo - at);  // below 2^31: the host limits a row's tiles
                     begin.row = r;
@@ -370,7 +373,6 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
     if (warp == CONSUMERS) {
         // ---- copies: the whole warp walks, lane b looks up the page of box b and issues its copies ----
         const uint64_t once = policy_evict_first();
-        int4 note = make_int4(-1, 0, 0, 0);  // row and unit that begin here and go on, the block of their last part
         uint32_t it = 0;
         while (w.left > 0) {
             const int n = a.len[w.row], sq = a.seq ? a.seq[w.row] : w.row;
@@ -406,14 +408,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                     tma_load_3d(dst + G::KV_BYTES, &maps.v, 0, at, column, &full[stage], once);
                 }
             }
-            if (end < w.tiles && from == 0) {
-                // it begins here, ends this run and goes on: its last tile lies that far behind the run's end
-                const Cut cut = whole_cut;
-                note = make_int4(w.row, w.unit, cut.run_of(cut.begin(blockIdx.x + 1) + w.tiles - end - 1), 0);
-            }
             if (w.left > 0) walk_next_piece<TILE>(a, w);
         }
-        if (lane == 0) reinterpret_cast<int4*>(a.work + (size_t)gridDim.x * 2 * part_floats(HB * a.chunk, DH))[blockIdx.x] = note;
         // rows without tiles: an empty one has nothing to attend to and gets zeros
         for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
             const int n = a.len[r], sq = a.seq ? a.seq[r] : r;
@@ -649,54 +645,101 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
     __syncthreads();
 }
 
-// Joins the parts of the (row, unit)s that were cut. One begins in some block of the first kernel (its
-// place 1) and goes on in the blocks after it (their place 0); that block's note says up to which. The
-// items are the query heads of these; a warp takes one at a time, or a whole block where items are
-// few. The order of the sums is fixed by the cut alone. All of this is a chain of a few trips to L2 behind the
-// first kernel's end, so the code is kept short: unrolled further it took longer to fetch than to run.
+// Joins the parts of the (row, unit)s that were cut. One begins in some run of the first kernel (place 1 of
+// its block's parts) and goes on in the runs after it (their place 0). Which these are follows from the
+// lengths, so every block finds them out while the first kernel still runs, and waits for that only to read
+// the parts (1500 tokens 9.0 -> 8.2 us, against notes that the first kernel left). The items are the query heads
+// of these; a warp takes one at a time, or a whole block where items are few. The order of the sums is fixed by
+// the cut alone. What follows the wait is a chain of trips to L2, so the code is kept short: unrolled further it
+// took longer to fetch than to run. (With 64 registers its blocks would fit beside running ones of the first
+// kernel, and cost that 2 us.)
 constexpr int JOIN_WARPS = 16, JOIN_BLOCKS = 148;
 
 template <int DH>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_paged_join_kernel(const __grid_constant__ PagedArgs a, int blocks, int HB) {
-    constexpr int E = DH / 128, U = 6;  // parts in flight per warp
-    __shared__ int4 notes[MAX_BLOCKS];
-    __shared__ int begins[MAX_BLOCKS], base[JOIN_WARPS];
+    constexpr int E = DH / 128, U = 4, THREADS = JOIN_WARPS * 32;  // U: parts in flight per warp
+    __shared__ int4 cuts[MAX_BLOCKS];  // row, unit, first run, last run
+    __shared__ int base[JOIN_WARPS];
+    __shared__ long long upto[THREADS], warp_sums[JOIN_WARPS];
     __shared__ __align__(16) float sums[JOIN_WARPS][DH];
     __shared__ float2 pairs[JOIN_WARPS];
     grid_dep_trigger();
-    grid_dep_sync();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int heads = HB * a.chunk;
+    const int heads = HB * a.chunk, tile = SLICE * CONSUMERS / HB;
     const size_t floats = part_floats(heads, DH);
-    const int4* src = reinterpret_cast<const int4*>(a.work + (size_t)blocks * 2 * floats);
-    // the blocks in which one begins, in a list
+    // tiles up to the end of every thread's rows
+    const int per = (a.rows + THREADS - 1) / THREADS;
+    int most = 0;
+    {
+        long long mine = 0;
+        for (int r = min(tid * per, a.rows), end = min(r + per, a.rows); r < end; r++) {
+            int tiles;
+            mine += row_tiles<true>(a, r, tile, tiles);
+            most = max(most, tiles);
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, mine, o);
+            if (lane >= o) mine += x;
+        }
+        if (lane == 31) warp_sums[warp] = mine;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < JOIN_WARPS; w++)
+            if (w < warp) mine += warp_sums[w];
+        upto[tid] = mine;
+        __syncthreads();
+    }
+    const Cut cut(upto[THREADS - 1], blocks, (long long)a.rows * a.units);
+    // thread b: whether run b ends within a (row, unit) that begins in it; their list
     int count = 0;
-    for (int j0 = 0; j0 < blocks; j0 += JOIN_WARPS * 32) {
-        const int j = j0 + tid;
-        const int4 note = j < blocks ? src[j] : make_int4(-1, 0, 0, 0);
-        const uint32_t all = __ballot_sync(0xffffffffu, note.x >= 0);
+    // (runs and rows of one tile each: none)
+    if (__syncthreads_or(most > 1 || cut.runs < cut.total)) {
+        int4 found = make_int4(-1, 0, 0, 0);
+        if (tid < cut.runs - 1) {
+            const long long t = cut.begin(tid + 1);
+            int c = 0;  // the thread whose rows hold tile t
+            for (int step = 1 << (31 - __clz((a.rows + per - 1) / per)); step; step /= 2)
+                if (upto[c + step - 1] <= t) c += step;
+            long long at = c ? upto[c - 1] : 0;
+            for (int r = c * per; r < a.rows; r++) {
+                int tiles;
+                long long n;
+                if (per == 1)
+                    n = upto[c] - at, tiles = (int)n / a.units;  // below 2^31: the host limits a row's tiles
+                else
+                    n = row_tiles<true>(a, r, tile, tiles);
+                if (at + n <= t) {
+                    at += n;
+                    continue;
+                }
+                const int in_row = (int)(t - at), of = in_row % tiles;
+                if (of > 0 && t - of >= cut.begin(tid)) found = make_int4(r, in_row / tiles, tid, cut.run_of(t - of + tiles - 1));
+                break;
+            }
+        }
+        const uint32_t all = __ballot_sync(0xffffffffu, found.x >= 0);
         if (lane == 0) base[warp] = __popc(all);
         __syncthreads();
-        int at = count;
+        int at = __popc(all & ((1u << lane) - 1));
+#pragma unroll
         for (int w = 0; w < JOIN_WARPS; w++) {
             if (w < warp) at += base[w];
             count += base[w];
         }
-        if (note.x >= 0) {
-            notes[j] = note;
-            begins[at + __popc(all & ((1u << lane) - 1))] = j;
-        }
+        if (found.x >= 0) cuts[at] = found;
         __syncthreads();
     }
+    grid_dep_sync();
     const int items = count * heads;
     const bool together = items <= 2 * (int)gridDim.x;
     const int width = together ? 1 : JOIN_WARPS;
     for (int item = blockIdx.x * width + (together ? 0 : warp); item < items; item += gridDim.x * width) {
-        const int b = begins[item / heads], slot = item % heads, of = slot / a.chunk, i = slot % a.chunk;
-        const int4 note = notes[b];
-        const int hk = note.y / a.chunks * HB + of, h0 = note.y % a.chunks * a.chunk;
+        const int4 piece = cuts[item / heads];
+        const int slot = item % heads, of = slot / a.chunk, i = slot % a.chunk;
+        const int hk = piece.y / a.chunks * HB + of, h0 = piece.y % a.chunks * a.chunk;
         if (i >= min(a.chunk, a.group - h0)) continue;
-        const size_t at = ((size_t)note.x * a.Hq + (size_t)hk * a.group + h0 + i) * DH;
+        const size_t at = ((size_t)piece.x * a.Hq + (size_t)hk * a.group + h0 + i) * DH;
         float m = -INFINITY, l = 0.f;
         float4 acc[E] = {};
         uint2 gate[E] = {};
@@ -705,15 +748,15 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_paged_join_kernel(const 
             for (int e = 0; e < E; e++) gate[e] = __ldg(reinterpret_cast<const uint2*>(a.gate + at + e * 128 + lane * 4));
         }
         const int stride = together ? JOIN_WARPS : 1;
-        for (int p0 = b + (together ? warp : 0); p0 <= note.z; p0 += U * stride) {
+        for (int p0 = piece.z + (together ? warp : 0); p0 <= piece.w; p0 += U * stride) {
             float2 ml[U];
             float4 x[U][E];
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int p = p0 + u * stride;
                 ml[u] = make_float2(-INFINITY, 0.f);
-                if (p <= note.z) {
-                    const float* part = a.work + ((size_t)p * 2 + (p == b)) * floats;
+                if (p <= piece.w) {
+                    const float* part = a.work + ((size_t)p * 2 + (p == piece.z)) * floats;
                     ml[u] = reinterpret_cast<const float2*>(part + (size_t)heads * DH)[slot];
 #pragma unroll
                     for (int e = 0; e < E; e++) x[u][e] = *reinterpret_cast<const float4*>(part + (size_t)slot * DH + e * 128 + lane * 4);
@@ -728,7 +771,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_paged_join_kernel(const 
             for (int e = 0; e < E; e++) acc[e].x *= f, acc[e].y *= f, acc[e].z *= f, acc[e].w *= f;
 #pragma unroll
             for (int u = 0; u < U; u++)
-                if (p0 + u * stride <= note.z) {
+                if (p0 + u * stride <= piece.w) {
                     const float c = exp2f(ml[u].x - off);
                     l += ml[u].y * c;
 #pragma unroll
@@ -859,7 +902,7 @@ extern "C" int s1_attn_prep_paged(const void* qg, const void* kr, const void* vr
 extern "C" size_t s1_attention_paged_workspace_floats(int Hq, int Hk, int Dh) {
     if (Hq <= 0 || Hk <= 0 || Hq % Hk != 0 || (Dh != 128 && Dh != 256)) return 0;
     const int group = Hq / Hk, chunks = (group + MAX_GROUP - 1) / MAX_GROUP;
-    return (size_t)MAX_BLOCKS * (2 * part_floats(head_block(Hk) * ((group + chunks - 1) / chunks), Dh) + 4);
+    return (size_t)MAX_BLOCKS * 2 * part_floats(head_block(Hk) * ((group + chunks - 1) / chunks), Dh);
 }
 
 extern "C" int s1_attention_paged(const void* q, const void* gate, void* out, const void* k_pages, const void* v_pages,

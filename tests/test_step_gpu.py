@@ -547,7 +547,7 @@ def test_paged_attention_cut_over_many_blocks(cs1, stream, Dh, Hq, Hk, page, len
 
 
 @pytest.mark.parametrize("Hq,Hk,tile,tiles", [(Hq, Hk, tile, tiles) for Hq, Hk, tile in ((8, 4, 16), (6, 2, 32), (3, 1, 64))
-                                              for tiles in (95, 96, 97, 191, 767, 768, 769, 2367, 2369) if tiles * tile < 80000])
+                                              for tiles in (63, 64, 65, 95, 97, 191, 511, 512, 513, 769, 2367, 2369) if tiles * tile < 80000])
 def test_paged_attention_where_runs_grow(cs1, stream, Hq, Hk, tile, tiles):
     """One row at the tile counts where its runs go from one tile to eight, and from there to one per block."""
     for n in (tiles * tile, tiles * tile - tile + 1):
