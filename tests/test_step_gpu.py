@@ -969,3 +969,27 @@ def test_cache_writes_reach_the_attention_launched_as_its_dependent(cs1, stream)
         if want is None:
             want = got
         assert (got == want).all()
+
+
+@pytest.mark.parametrize("mode", [0, 1])
+def test_lengths_written_by_the_kernel_before(cs1, stream, mode):
+    """Attentions queued without a wait, each behind a kernel that changes the lengths it is cut by: each as alone."""
+    Hq, Hk, Dh, page = 8, 4, 128, 16
+    sets = [[3000, 1, 700, 0], [1, 4000, 16, 2500], [0, 33, 0, 1], [2048, 2048, 2048, 2048]]
+    c = attn_case([max(s[i] for s in sets) for i in range(4)], Hq, Hk, Dh, page, 11)
+    want = [run_attn(cs1, stream, dict(c, lens=s), True, Dh ** -0.5) for s in sets]
+    d = {m: up(c[m], stream) for m in ("q", "gate", "kp", "vp", "table")}
+    lens, floats = ints([sets[0]] + sets, stream), cs1.s1_attention_paged_workspace_floats(Hq, Hk, Dh)     # page 0: the live ones
+    ws, pool = L.DeviceBuffer(floats * 4), (C.c_void_p * 1)(lens.ptr.value)
+    order = [1, 0, 3, 2, 0, 2, 1, 3] * 4
+    outs = [L.DeviceBuffer(4 * Hq * Dh * 2) for _ in order]
+    stream.sync()
+    before = cs1.s1_set_dependent_launch(mode)
+    for k, out in zip(order, outs):
+        src, dst = np.array([k + 1], np.int32), np.array([0], np.int32)
+        L.check(cs1.s1_pages_copy(pool, 1, 5, 16, src.ctypes.data, dst.ctypes.data, 1, stream.handle), "lengths")
+        L.check(cs1.s1_attention_paged(d["q"].at(), d["gate"].at(), out.at(), d["kp"].at(), d["vp"].at(), len(c["kp"]), page, d["table"].at(),
+                                       c["table"].shape[1], 4, None, lens.at(), 4, Hq, Hk, Dh, Dh ** -0.5, ws.at(), floats, stream.handle), "attention")
+    cs1.s1_set_dependent_launch(before)
+    for k, out in zip(order, outs):
+        assert (down(out, (4, Hq, Dh), stream) == want[k]).all()
