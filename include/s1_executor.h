@@ -154,12 +154,14 @@ int s1_attn_prep_paged(const void* qg, const void* kr, const void* vr, int ld, c
 
 /* Attention of one new token per row: q, out [rows, Hq, Dh], row r over the first len[r] tokens of
  * sequence seq[r] (null: r), its own one among them; several rows of one sequence with growing len
- * are a causal window. gate (nullable) [rows, Hq, Dh]: out = o * sigmoid(gate). len 0: zeros; len
- * negative: the row sits out, out is left as it is. A row with a page outside the pools comes out
- * undefined (code 32), a row that the table does not have is left as it is (code 31); a row whose scores are all -inf comes out
- * as zeros. page_tokens a multiple of 16, Dh 128 or 256, Hq a multiple of Hk, at most 2^20 rows; 16-byte
- * aligned pointers. Two launches; the result does not depend on
- * what else runs, only on the lengths of the call (they decide where the cache is cut). The workspace (at least
+ * are a causal window. Neighbouring rows of a window, each at most 16 tokens longer than the one before, read a
+ * large cache once for as many of them as have 16 query heads per key-value head together, in calls with
+ * more rows than sequences and at most 8192 rows. gate (nullable) [rows, Hq, Dh]: out = o * sigmoid(gate). len 0:
+ * zeros; len negative: the row sits out, out is left as it is. A row with a page outside the pools comes out
+ * undefined (code 32), a row that the table does not have is left as it is (code 31); a row whose scores
+ * are all -inf comes out as zeros. page_tokens a multiple of 16, Dh 128 or 256, Hq a multiple of Hk, at
+ * most 2^20 rows; 16-byte aligned pointers. Two launches; the result does not depend on what else
+ * runs, only on the call itself (its lengths and shapes decide where the cache is cut). The workspace (at least
  * s1_attention_paged_workspace_floats; 0 for shapes that the operator does not take) needs no
  * clearing and belongs to one call at a time. */
 size_t s1_attention_paged_workspace_floats(int Hq, int Hk, int Dh);

@@ -269,7 +269,8 @@ def test_paged_attention_refuses(cs1, bad):
 
 def test_paged_attention_workspace(cs1):
     f = cs1.s1_attention_paged_workspace_floats
-    assert 0 < f(4, 4, 128) < f(16, 4, 128) < f(16, 4, 256)
+    assert 0 < f(24, 4, 128) < f(16, 4, 128) and f(24, 4, 256) < f(16, 4, 256)      # rows of a product: 2 * 6 and 4 * 4
+    assert max(f(q, k, d) for q in range(1, 65) for k in range(1, q + 1) for d in (128, 256)) < 5 << 20
     assert f(16, 1, 256) == f(32, 1, 256)          # more than 16 heads of one key-value head go in parts
     assert f(4, 3, 128) == f(0, 1, 128) == f(4, 0, 128) == f(4, 4, 64) == 0
 

@@ -573,6 +573,80 @@ def test_paged_attention_rows_of_one_sequence_are_a_causal_window(cs1, stream):
     assert (run_attn(cs1, stream, one, True, 128 ** -0.5) == run_attn(cs1, stream, c, True, 128 ** -0.5)[4:5]).all()
 
 
+def windows_of(spec):
+    """Rows of (sequence, first length, rows, growth) windows."""
+    lens = [n + i * grow for _, n, rows, grow in spec for i in range(rows)]
+    return lens, [q for q, _, rows, _ in spec for _ in range(rows)]
+
+
+def wide(c):
+    """The case with a table that could hold 70 MB: rows of one sequence share tiles in such caches."""
+    n, w = c["table"].shape
+    more = max(0, int(70e6 / (n * c["page"] * c["Hk"] * c["Dh"] * 4)) + 1 - w)
+    return dict(c, table=np.concatenate([c["table"], np.full((n, more), -1, c["table"].dtype)], 1))
+
+
+@pytest.mark.parametrize("Dh", [128, 256])
+@pytest.mark.parametrize("Hq,Hk", [(24, 4), (16, 4), (16, 2), (8, 8), (5, 1), (12, 1), (40, 2), (6, 2), (9, 3)])
+@pytest.mark.parametrize("spec", [
+    [(0, 1, 3, 1), (1, 14, 5, 1), (2, 100, 1, 1), (3, 60, 17, 1)],                     # from the first token on; over a tile's end
+    [(0, 500, 3, 1), (0, 503, 2, 1), (1, 503, 3, 1), (1, 400, 3, 1), (2, 2000, 9, 1)],  # two windows of one sequence, a shorter one behind
+    [(0, 300, 4, 0), (1, 64, 4, 16), (2, 64, 4, 17), (3, 129, 2, 1), (3, -1, 2, 0), (3, 131, 2, 1), (4, 0, 3, 0), (4, 1, 2, 0)],
+    [(0, 40, 70, 1), (1, 700, 49, 1), (2, 9, 1, 1)]])                                  # longer than rows look back
+def test_paged_attention_windows_share_tiles(cs1, stream, Dh, Hq, Hk, spec):
+    """Rows of one sequence, as many at once as fit a product: each over its own length, those that sit out left alone."""
+    lens, seq = windows_of(spec)
+    c = wide(attn_case(lens, Hq, Hk, Dh, 32, Hq + Dh, seq=seq))
+    got = run_attn(cs1, stream, c, True, Dh ** -0.5)
+    check_attn(c, got, True, Dh ** -0.5)
+    assert (run_attn(cs1, stream, c, True, Dh ** -0.5, ws_fill=0) == got).all()
+
+
+@pytest.mark.parametrize("Dh,Hq,Hk", [(128, 16, 4), (128, 8, 8), (256, 12, 2), (128, 5, 1)])
+def test_paged_attention_windows_cut_over_many_blocks(cs1, stream, Dh, Hq, Hk):
+    lens, seq = windows_of([(0, 9000, 5, 1), (1, 3, 2, 1), (2, 4000, 3, 5), (3, 2500, 16, 1)])
+    c = wide(attn_case(lens, Hq, Hk, Dh, 64, Hq, seq=seq))
+    check_attn(c, run_attn(cs1, stream, c, False, Dh ** -0.5), False, Dh ** -0.5)
+
+
+@pytest.mark.parametrize("Dh,Hq,Hk", [(128, 16, 4), (128, 8, 8), (256, 16, 4), (128, 4, 1), (256, 6, 2)])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_paged_attention_a_window_keeps_later_tokens_from_earlier_rows(cs1, stream, Dh, Hq, Hk, bad):
+    """What only the later rows of a window may see is infinite or NaN: the earlier ones do not change."""
+    lens, seq = windows_of([(0, 190, 8, 1), (1, 30, 4, 5), (2, 47, 4, 1)])
+    c = wide(attn_case(lens, Hq, Hk, Dh, 16, 7, seq=seq))
+    clean = run_attn(cs1, stream, c, True, Dh ** -0.5)
+    hurt = dict(c, kp=c["kp"].copy(), vp=c["vp"].copy())
+    first = {0: 194, 1: 36, 2: 48}   # the first token that is hurt
+    for s, t0 in first.items():
+        for t in range(t0, max(n for n, q in zip(lens, seq) if q == s)):
+            for m in ("kp", "vp"):
+                hurt[m][c["table"][s, t // 16], t % 16] = bf(np.full((Hk, Dh), bad))
+    got = run_attn(cs1, stream, hurt, True, Dh ** -0.5)
+    early = [r for r in range(len(lens)) if lens[r] <= first[seq[r]]]
+    assert 6 < len(early) < len(lens)
+    assert (got[early] == clean[early]).all()
+    if np.isnan(bad):
+        assert np.isnan(f32(got[[r for r in range(len(lens)) if r not in early]])).all()
+
+
+def test_paged_attention_windows_refuse_rows_on_the_device(cs1, stream):
+    """Rows without a sequence, or past their table, between rows that share tiles; more rows than sequences and no list of them."""
+    lens, seq = windows_of([(0, 190, 3, 1), (1, 30, 4, 1), (2, 47, 4, 1)])
+    c = wide(attn_case(lens, 16, 4, 128, 16, 7, seq=seq))
+    longest = c["table"].shape[1] * 16
+    for r, (s, n) in {1: (-1, 191), 4: (3, 31), 5: (1, longest + 1), 8: (2 ** 31 - 1, 48)}.items():
+        hurt = dict(c, seq=list(c["seq"]), lens=list(c["lens"]))
+        hurt["seq"][r], hurt["lens"][r] = s, n
+        got = run_attn(cs1, stream, hurt, True, 128 ** -0.5)
+        assert status() == (0, 31, 0)
+        assert (got[r] == 0x4242).all()
+        rest = [i for i in range(len(lens)) if i != r]
+        check_attn(c, got, True, 128 ** -0.5, rest)
+    got = run_attn(cs1, stream, dict(c, seq=None, lens=[190, 30, 47] + [5] * 8), True, 128 ** -0.5)
+    assert status() == (0, 31, 0) and (got[3:] == 0x4242).all() and (got[:3] != 0x4242).any()
+
+
 @pytest.mark.parametrize("climb", [0.0, 0.4, -0.4, 30.0])
 def test_paged_attention_with_scores_that_climb(cs1, stream, climb):
     """Scores that grow or fall along the cache by up to several hundred: the running maximum moves in every tile, or never."""
