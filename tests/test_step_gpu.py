@@ -630,6 +630,20 @@ def test_paged_attention_a_window_keeps_later_tokens_from_earlier_rows(cs1, stre
         assert np.isnan(f32(got[[r for r in range(len(lens)) if r not in early]])).all()
 
 
+@pytest.mark.parametrize("rows", [513, 2999, 8191, 8192, 8193])
+def test_paged_attention_windows_of_many_rows(cs1, stream, rows):
+    """More rows than a block has threads, in windows of 1 to 40 rows: up to 8192 they share tiles, above they do not."""
+    spec, left, i = [], rows, 0
+    while left:
+        n = min(left, (3, 1, 7, 40, 2, 4, 16)[i * i % 7])
+        spec.append((i, 1 + (i * 37) % 90, n, 1))
+        left, i = left - n, i + 1
+    lens, seq = windows_of(spec)
+    c = wide(attn_case(lens, 8, 2, 128, 16, rows, seq=seq))
+    got = run_attn(cs1, stream, c, True, 128 ** -0.5)
+    check_attn(c, got, True, 128 ** -0.5, list(range(0, rows, 41)) + list(range(rows - 45, rows)))
+
+
 def test_paged_attention_windows_refuse_rows_on_the_device(cs1, stream):
     """Rows without a sequence, or past their table, between rows that share tiles; more rows than sequences and no list of them."""
     lens, seq = windows_of([(0, 190, 3, 1), (1, 30, 4, 1), (2, 47, 4, 1)])
