@@ -146,7 +146,7 @@ int s1_gdn_conv_gates_step(const void* qkv, int ld, const void* w, void* q, void
  * tables cos, sin [angles, half] are read at row angle[r] (null: at pos[r]), so tables of one row per
  * packed row serve positions on several axes. Rows at one place of the cache are refused: their q
  * and gate come out, the place is left as it is. Any page_tokens; 16-byte aligned pointers; at most
- * 65536 rows (each is compared with every other). */
+ * 65536 rows. */
 int s1_attn_prep_paged(const void* qg, const void* kr, const void* vr, int ld, const void* qw, const void* kw,
                        const void* cos, const void* sin, int angles, const int* angle, void* q, void* gate, void* k_pages,
                        void* v_pages, int n_pages, int page_tokens, const int* table, int table_pages, int n_seqs,

@@ -40,75 +40,47 @@ struct PrepArgs {
     int ld, angles, rows, Hq, Hk, half;
     float eps;
     PageTable table;
+    uint32_t by_page;  // p / page_tokens = p * by_page >> page_shift for p < 2^30, more than any table holds
+    int page_shift;
+    int per;           // rows of a block
     int* error;
 };
 
-constexpr int PREP_THREADS = 256;
+constexpr int PREP_THREADS = 256, PREP_ROWS = 128, MANY_ROWS = 512;
 
-// DH / 8 lanes per head, 8 consecutive dims per lane; the rotary partner of dim d (d +- half) lives
-// half / 8 lanes away. A row's units are its Hq query heads, Hk key heads and Hk value heads. Latency bounds it:
-// 251 rows of 16 and 4 heads of 256 (10 MB) take 5.2 us, one row 2.3, launch and all.
+__device__ __forceinline__ int page_slot(const PrepArgs& a, int p) { return (int)((uint64_t)(uint32_t)p * a.by_page >> a.page_shift); }
+// The page of a place, -1: the table has none.
+__device__ __forceinline__ int page_of(const PrepArgs& a, int r, int p) {
+    const int sq = a.seq ? a.seq[r] : r, slot = page_slot(a, p);
+    if (p < 0 || p >= 1 << 30 || sq < 0 || sq >= a.table.sequences || slot >= a.table.width) return -1;
+    return a.table.pages[(size_t)sq * a.table.width + slot];
+}
+
+// DH / 8 lanes per head, 8 consecutive dims per lane; the rotary partner of dim d (d +- half) lives half / 8 lanes
+// away. A row's units are its Hq query heads, Hk key heads and Hk value heads.
 template <int DH>
-__global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __grid_constant__ PrepArgs a) {
-    constexpr int LANES = DH / 8, UNITS = PREP_THREADS / LANES;
-    grid_dep_trigger();
-    grid_dep_sync();
-    // A row is a few hundred instructions behind three trips to memory, so whatever does not depend on an
-    // earlier trip is asked for at once: row, weights and positions, then page and rotary rows, then the rest.
-    const int r = blockIdx.x, tid = threadIdx.x;
-    const int unit0 = blockIdx.y * UNITS;
-    const int heads = a.Hq + 2 * a.Hk;
-    const int unit = min(unit0 + tid / LANES, heads - 1);
-    const bool live = unit0 + tid / LANES < heads, writes = unit0 + UNITS > a.Hq;
-    const int d0 = tid % LANES * 8;
-    const bool is_q = unit < a.Hq, is_v = unit >= a.Hq + a.Hk;
-    const int h = is_q ? unit : is_v ? unit - a.Hq - a.Hk : unit - a.Hq;
-    const bf16* src = is_q ? a.qg + (size_t)r * a.ld + (size_t)h * 2 * DH : (is_v ? a.vr : a.kr) + (size_t)r * a.ld + (size_t)h * DH;
-    const uint4 raw = ld16_stream(src + d0), weight = ld16((is_q ? a.qw : a.kw) + d0);
-    const uint4 gate = is_q ? ld16_stream(src + DH + d0) : make_uint4(0, 0, 0, 0);
-    const int p = a.pos[r], sq = a.seq ? a.seq[r] : r;
-    const int turn = a.angle ? a.angle[r] : p;
-    const int pt = a.table.page_tokens;
-    auto place_of = [&](int row, int pos, int& seq) {  // entry of the page table, -1: the table has none
-        seq = a.seq ? a.seq[row] : row;
-        return pos >= 0 && seq >= 0 && seq < a.table.sequences && pos / pt < a.table.width ? pos / pt : -1;
-    };
-    int pj = writes && tid < a.rows ? a.pos[tid] : -1;
-    if (p < 0) return;  // the row sits out
-    const int slot = p / pt, off = p - slot * pt;
-    int code = 0, page = -1;
-    if (sq < 0 || sq >= a.table.sequences || slot >= a.table.width)
-        code = PAGED_BAD_ROW;
-    else if (turn < 0 || turn >= a.angles)
-        code = PAGED_BAD_ANGLE;
-    else
-        page = a.table.pages[(size_t)sq * a.table.width + slot];
-    const int rot = 2 * a.half;
-    uint4 turns[2] = {};
-    if (d0 < rot && code == 0) {
-        // half is a multiple of 8, so the 8 dims of a lane share one aligned table pack
-        turns[0] = ld16(a.cos + (size_t)turn * a.half + d0 % a.half);
-        turns[1] = ld16(a.sin + (size_t)turn * a.half + d0 % a.half);
+struct PrepUnit {
+    static constexpr int LANES = DH / 8, UNITS = PREP_THREADS / LANES;
+    int d0, h;
+    bool live, is_q, is_v, writes;  // writes: the block has key or value heads
+    __device__ explicit PrepUnit(const PrepArgs& a) {
+        const int unit0 = blockIdx.y * UNITS, heads = a.Hq + 2 * a.Hk;
+        const int unit = min(unit0 + (int)threadIdx.x / LANES, heads - 1);
+        live = unit0 + (int)threadIdx.x / LANES < heads, writes = unit0 + UNITS > a.Hq;
+        d0 = threadIdx.x % LANES * 8;
+        is_q = unit < a.Hq, is_v = unit >= a.Hq + a.Hk;
+        h = is_q ? unit : is_v ? unit - a.Hq - a.Hk : unit - a.Hq;
     }
-    // Two rows at one place of the cache would race: neither is written.
-    bool clash = false;
-    for (int j = tid; writes && j < a.rows; j += PREP_THREADS) {
-        if (j != tid) pj = a.pos[j];
-        if (j == r || pj < 0 || pj % pt != off) continue;
-        int sj;
-        const int slot_j = place_of(j, pj, sj);
-        clash |= slot_j >= 0 && a.table.pages[(size_t)sj * a.table.width + slot_j] == page;
+    __device__ const bf16* row(const PrepArgs& a, int r) const {
+        return is_q ? a.qg + (size_t)r * a.ld + (size_t)h * 2 * DH : (is_v ? a.vr : a.kr) + (size_t)r * a.ld + (size_t)h * DH;
     }
-    if (code == 0 && (page < 0 || page >= a.table.n_pages)) code = PAGED_BAD_PAGE;
-    if (code) {
-        if (tid == 0) atomicCAS(a.error, 0, code);
-        return;
-    }
-    if (writes && __syncthreads_or(clash)) {
-        if (tid == 0) atomicCAS(a.error, 0, PAGED_CLASH);
-        page = -1;
-    }
+    __device__ const bf16* weights(const PrepArgs& a) const { return is_q ? a.qw : a.kw; }
+};
 
+template <int DH>
+__device__ __forceinline__ void unit_out(const PrepArgs& a, const PrepUnit<DH>& u, int r, uint4 raw, uint4 weight, uint4 gate,
+                                         const uint4 (&turns)[2], int page, int off) {
+    constexpr int LANES = DH / 8;
     float x[8], wv[8], y[8], cs[8], sn[8];
     unpack8(raw, x);
     unpack8(weight, wv);
@@ -124,18 +96,159 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __g
     for (int i = 0; i < 8; i++) {
         const float partner = __shfl_xor_sync(0xffffffffu, x[i], a.half / 8);
         y[i] = x[i];
-        if (d0 < rot) y[i] = x[i] * cs[i] + (d0 < a.half ? -partner : partner) * sn[i];
+        if (u.d0 < 2 * a.half) y[i] = x[i] * cs[i] + (u.d0 < a.half ? -partner : partner) * sn[i];
     }
-    if (!live) return;
-    if (is_q) {
-        st16(a.q + ((size_t)r * a.Hq + h) * DH + d0, pack8(y));
-        st16(a.gate + ((size_t)r * a.Hq + h) * DH + d0, gate);
+    if (!u.live) return;
+    if (u.is_q) {
+        st16(a.q + ((size_t)r * a.Hq + u.h) * DH + u.d0, pack8(y));
+        st16(a.gate + ((size_t)r * a.Hq + u.h) * DH + u.d0, gate);
     } else if (page >= 0) {
-        const size_t at = (((size_t)page * a.table.page_tokens + off) * a.Hk + h) * DH + d0;
-        if (is_v)
+        const size_t at = (((size_t)page * a.table.page_tokens + off) * a.Hk + u.h) * DH + u.d0;
+        if (u.is_v)
             st16(a.v_pages + at, raw);
         else
             st16(a.k_pages + at, pack8(y));
+    }
+}
+
+// Latency bounds it: 251 rows of 16 and 4 heads of 256 (10 MB) take 5.0 us, one row 2.2, launch and all.
+template <int DH>
+__global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_kernel(const __grid_constant__ PrepArgs a) {
+    grid_dep_trigger();
+    grid_dep_sync();
+    // A row is a few hundred instructions behind three trips to memory, so whatever does not depend on an
+    // earlier trip is asked for at once: row, weights and positions, then page and rotary rows, then the rest.
+    const int r = blockIdx.x, tid = threadIdx.x;
+    const PrepUnit<DH> u(a);
+    const bf16* src = u.row(a, r);
+    const uint4 raw = ld16_stream(src + u.d0), weight = ld16(u.weights(a) + u.d0);
+    const uint4 gate = u.is_q ? ld16_stream(src + DH + u.d0) : make_uint4(0, 0, 0, 0);
+    const int p = a.pos[r], sq = a.seq ? a.seq[r] : r;
+    const int turn = a.angle ? a.angle[r] : p;
+    const int pt = a.table.page_tokens;
+    int pj = u.writes && tid < a.rows ? a.pos[tid] : -1;
+    if (p < 0) return;  // the row sits out
+    const int slot = page_slot(a, p), off = p - slot * pt;
+    int code = 0, page = -1;
+    if (p >= 1 << 30 || sq < 0 || sq >= a.table.sequences || slot >= a.table.width)
+        code = PAGED_BAD_ROW;
+    else if (turn < 0 || turn >= a.angles)
+        code = PAGED_BAD_ANGLE;
+    else
+        page = a.table.pages[(size_t)sq * a.table.width + slot];
+    uint4 turns[2] = {};
+    if (u.d0 < 2 * a.half && code == 0) {
+        // half is a multiple of 8, so the 8 dims of a lane share one aligned table pack
+        turns[0] = ld16(a.cos + (size_t)turn * a.half + u.d0 % a.half);
+        turns[1] = ld16(a.sin + (size_t)turn * a.half + u.d0 % a.half);
+    }
+    // Two rows at one place of the cache would race: neither is written.
+    bool clash = false;
+    for (int j = tid; u.writes && j < a.rows; j += PREP_THREADS) {
+        if (j != tid) pj = a.pos[j];
+        if (j == r || pj < 0 || pj >= 1 << 30 || pj - page_slot(a, pj) * pt != off) continue;
+        const int other = page_of(a, j, pj);
+        clash |= other >= 0 && other == page;
+    }
+    if (code == 0 && (page < 0 || page >= a.table.n_pages)) code = PAGED_BAD_PAGE;
+    if (code) {
+        if (tid == 0) atomicCAS(a.error, 0, code);
+        return;
+    }
+    if (u.writes && __syncthreads_or(clash)) {
+        if (tid == 0) atomicCAS(a.error, 0, PAGED_CLASH);
+        page = -1;
+    }
+
+    unit_out<DH>(a, u, r, raw, weight, gate, turns, page, off);
+}
+
+// Many rows: a block takes `per` of them and looks all others up among these, by a hash of their places in the
+// cache; each row against each other by itself took longer than all the rest (8192 rows 223 us, 65536 13.9 ms). The
+// next row is asked for while one is worked on. Measured, 24 and 4 heads of 128: 1000 rows 10.4 us (one row a block: 12.9),
+// 8192: 69 (223), 65536: 538 (13.9 ms; the bytes alone 287); up to 512 rows one row a block is as quick (6.3 us).
+// (rows / 512 of them a block; rows / 1024: 76 and 602, rows / 256: 70 and 538.)
+template <int DH>
+__global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_many_kernel(const __grid_constant__ PrepArgs a) {
+    constexpr int HASH = 512, AT_ONCE = 4;
+    __shared__ int first[HASH], next[PREP_ROWS], places[PREP_ROWS];  // chains of 1 + the row in the block; its place, -1: none
+    __shared__ bool clashes[PREP_ROWS];
+    grid_dep_trigger();
+    grid_dep_sync();
+    const PrepUnit<DH> u(a);
+    const int tid = threadIdx.x, pt = a.table.page_tokens;
+    const int r0 = blockIdx.x * a.per, n = min(a.per, a.rows - r0);
+    auto place_of = [&](int r, int p) {
+        const int page = page_of(a, r, p);
+        return page >= 0 && page < a.table.n_pages ? page * pt + p - page_slot(a, p) * pt : -1;
+    };
+    auto hash = [](int place) { return (uint32_t)place * 2654435769u >> 23; };
+    if (u.writes) {
+        for (int i = tid; i < HASH; i += PREP_THREADS) first[i] = 0;
+        __syncthreads();
+        if (tid < n) {
+            places[tid] = place_of(r0 + tid, a.pos[r0 + tid]);
+            clashes[tid] = false;
+            if (places[tid] >= 0) next[tid] = atomicExch(&first[hash(places[tid])], tid + 1);
+        }
+        __syncthreads();
+        for (int j0 = tid; j0 < a.rows; j0 += AT_ONCE * PREP_THREADS) {
+            int place[AT_ONCE];
+#pragma unroll
+            for (int e = 0; e < AT_ONCE; e++) {
+                const int j = min(j0 + e * PREP_THREADS, a.rows - 1);
+                place[e] = place_of(j, a.pos[j]);
+            }
+#pragma unroll
+            for (int e = 0; e < AT_ONCE; e++) {
+                const int j = min(j0 + e * PREP_THREADS, a.rows - 1);
+                if (place[e] < 0) continue;
+                for (int i = first[hash(place[e])]; i > 0; i = next[i - 1])
+                    if (places[i - 1] == place[e] && r0 + i - 1 != j) clashes[i - 1] = true;
+            }
+        }
+        __syncthreads();
+    }
+    const uint4 weight = ld16(u.weights(a) + u.d0);
+    uint4 raw, gate = make_uint4(0, 0, 0, 0);
+    int p;
+    auto ask = [&](int r) {
+        const bf16* src = u.row(a, r);
+        raw = ld16_stream(src + u.d0);
+        if (u.is_q) gate = ld16_stream(src + DH + u.d0);
+        p = a.pos[r];
+    };
+    ask(r0);
+#pragma unroll 1
+    for (int i = 0; i < n; i++) {
+        const int r = r0 + i, at = p;
+        const uint4 raw_now = raw, gate_now = gate;
+        if (i + 1 < n) ask(r + 1);
+        if (at < 0) continue;  // sits out
+        const int sq = a.seq ? a.seq[r] : r, turn = a.angle ? a.angle[r] : at;
+        int code = 0, page = -1;
+        uint4 turns[2] = {};
+        if (at >= 1 << 30 || sq < 0 || sq >= a.table.sequences || page_slot(a, at) >= a.table.width)
+            code = PAGED_BAD_ROW;
+        else if (turn < 0 || turn >= a.angles)
+            code = PAGED_BAD_ANGLE;
+        else {
+            page = page_of(a, r, at);
+            if (page < 0 || page >= a.table.n_pages) code = PAGED_BAD_PAGE;
+            if (u.d0 < 2 * a.half) {
+                turns[0] = ld16(a.cos + (size_t)turn * a.half + u.d0 % a.half);
+                turns[1] = ld16(a.sin + (size_t)turn * a.half + u.d0 % a.half);
+            }
+        }
+        if (code) {
+            if (tid == 0) atomicCAS(a.error, 0, code);
+            continue;
+        }
+        if (u.writes && clashes[i]) {
+            if (tid == 0) atomicCAS(a.error, 0, PAGED_CLASH);
+            page = -1;
+        }
+        unit_out<DH>(a, u, r, raw_now, weight, gate_now, turns, page, at - page_slot(a, at) * pt);
     }
 }
 
@@ -1014,14 +1127,18 @@ extern "C" int s1_attn_prep_paged(const void* qg, const void* kr, const void* vr
     a.k_pages = static_cast<bf16*>(k_pages), a.v_pages = static_cast<bf16*>(v_pages);
     a.angle = angle, a.seq = seq, a.pos = pos;
     a.ld = ld, a.angles = angles, a.rows = rows, a.Hq = Hq, a.Hk = Hk, a.half = half, a.eps = eps, a.table = t;
+    int shift = 31 - __builtin_clz(page_tokens);
+    a.page_shift = 31 + shift, a.by_page = (uint32_t)((1ULL << a.page_shift) / page_tokens + 1);
+    a.per = rows <= MANY_ROWS ? 1 : std::max(2, std::min(PREP_ROWS, rows / 512));
     const int units = PREP_THREADS / (Dh / 8);
-    const dim3 grid(rows, (Hq + 2 * Hk + units - 1) / units);
+    const dim3 grid((rows + a.per - 1) / a.per, (Hq + 2 * Hk + units - 1) / units);
     if (grid.y > 65535) return cudaErrorInvalidValue;
     int dev = 0;
     const int rc = error_word(&a.error, &dev);
     if (rc != 0) return rc;
-    const cudaError_t e = launch_dep(Dh == 256 ? attn_prep_paged_kernel<256> : attn_prep_paged_kernel<128>, grid, PREP_THREADS, 0,
-                                     as_stream(stream), a);
+    auto* const one = Dh == 256 ? attn_prep_paged_kernel<256> : attn_prep_paged_kernel<128>;
+    auto* const many = Dh == 256 ? attn_prep_paged_many_kernel<256> : attn_prep_paged_many_kernel<128>;
+    const cudaError_t e = launch_dep(a.per == 1 ? one : many, grid, PREP_THREADS, 0, as_stream(stream), a);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

@@ -429,6 +429,51 @@ def test_prep_refuses_rows_on_the_device(cs1, stream):
         assert (kp[~touched] == c["kp"][~touched]).all() and (vp[~touched] == c["vp"][~touched]).all()
 
 
+@pytest.mark.parametrize("rows,Dh,Hq,Hk,page", [(512, 128, 4, 2, 16), (513, 128, 4, 2, 16), (513, 256, 12, 2, 7), (700, 128, 20, 4, 64), (2100, 128, 1, 1, 1),
+                                                (3001, 256, 2, 1, 300), (9000, 128, 2, 1, 1024), (40001, 128, 1, 1, 48)])
+@pytest.mark.parametrize("hurt", [False, True])
+def test_prep_of_many_rows(cs1, stream, rows, Dh, Hq, Hk, page, hurt):
+    """A chunk of a prompt and more into the cache, whole; and with rows that sit out, are refused, or share a place."""
+    rng = np.random.default_rng(rows + hurt)
+    nseq, half, angles = 5, 16, 64
+    need = [-(-rows // nseq // page) + 1] * nseq
+    n_pages = sum(need) + 1
+    c = prep_inputs(rows, Hq, Hk, Dh, half, angles, n_pages, page, 0, rows)
+    table = make_table(need, n_pages, max(need) + 1, 3)
+    places = rng.permutation(nseq * need[0] * page)[:rows]           # no place twice
+    if not hurt:
+        places.sort()
+    seq, pos, angle = places // (need[0] * page), places % (need[0] * page), rng.integers(0, angles, rows)
+    lost = np.zeros(rows, bool)                                      # rows that leave nothing at all
+    if hurt:
+        table[4, 0] = table[3, 0]                                    # two sequences name one page
+        some = rng.permutation(rows)[:50].reshape(5, 10)
+        pos[some[0]], lost[some[0]] = -1 - rng.integers(0, 9, 10), True
+        seq[some[1]], lost[some[1]] = np.where(rng.random(10) < 0.5, -1, nseq), True
+        pos[some[2]], lost[some[2]] = np.array([max(need) * page, (max(need) + 1) * page, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1] * 2), True
+        angle[some[3]], lost[some[3]] = np.where(rng.random(10) < 0.5, -1, angles), True
+        other = rng.integers(0, rows, 10)
+        seq[some[4]], pos[some[4]] = seq[other], pos[other]          # twice at one place, or lost with the row copied
+        lost[some[4]] |= (pos[some[4]] < 0) | (seq[some[4]] < 0) | (seq[some[4]] >= nseq) | (pos[some[4]] >= max(need) * page)
+    q, gate, kp, vp = run_prep(cs1, stream, c, table, seq, pos, angle)
+    code = status()[1]
+    assert code in ((31, 32, 33, 34) if hurt else (0,))
+    (wq, tq), wg, (wk, tk), wv = prep_formula(c, np.clip(angle, 0, angles - 1))
+    assert (q[lost] == 0x4242).all() and (gate[lost] == 0x4242).all()
+    assert (np.abs(f32(q) - wq)[~lost] <= tq[~lost]).all() and (gate[~lost] == wg[~lost]).all()
+    # every row with a place in the table counts for it, one with a bad angle too
+    named = (pos >= 0) & (pos < table.shape[1] * page) & (seq >= 0) & (seq < nseq)
+    at = np.where(named, table[np.where(named, seq, 0), np.where(named, pos, 0) // page].astype(np.int64) * page + pos % page, -1)
+    held, count = np.unique(at[named], return_counts=True)
+    alone = np.isin(at, held[count == 1]) & ~lost
+    assert (count > 1).any() == hurt
+    kp2, vp2 = kp.reshape(-1, Hk, Dh), vp.reshape(-1, Hk, Dh)
+    assert (np.abs(f32(kp2[at[alone]]) - wk[alone]) <= tk[alone]).all() and (vp2[at[alone]] == wv[alone]).all()
+    rest = np.ones(len(kp2), bool)
+    rest[at[alone]] = False
+    assert (kp2[rest] == c["kp"].reshape(kp2.shape)[rest]).all() and (vp2[rest] == c["vp"].reshape(vp2.shape)[rest]).all()
+
+
 def test_prep_agrees_with_the_prefill_operator(cs1, stream):
     """The rows of cs1_attn_prep, within the bf16 steps of its roundings in between."""
     T, Hq, Hk, Dh, half, page = 37, 8, 2, 128, 32, 16
