@@ -47,7 +47,50 @@ __device__ __forceinline__ bool step_clash(const StepSeqs& s, int i, int in, int
     return clash;
 }
 
-// (At most 65535 sequences: a grid dimension, and every sequence is compared with every other.)
+// The same for `n` sequences of a block, i0 and on, at once: every other sequence's slots are looked up among theirs,
+// which for many sequences takes a fraction of comparing all with all in every block. All threads of the block call it.
+constexpr int STEP_ROWS = 128;
+struct StepLookup {
+    static constexpr int HASH = 512;
+    int first[HASH], next[2 * STEP_ROWS], slot[2 * STEP_ROWS];  // chains of 1 + entry; entries: outs, then ins
+    bool clashes[STEP_ROWS];
+    static __device__ __forceinline__ uint32_t hash(int s) { return (uint32_t)s * 2654435769u >> 23; }
+    template <int THREADS>
+    __device__ __forceinline__ void find(const StepSeqs& s, int i0, int n) {
+        const int tid = threadIdx.x;
+        for (int e = tid; e < HASH; e += THREADS) first[e] = 0;
+        __syncthreads();
+        for (int e = tid; e < 2 * n; e += THREADS) {
+            const int at = e < n ? e : STEP_ROWS + e - n;
+            slot[at] = e < n ? s.slot_out[i0 + e] : s.slot_in[i0 + e - n];
+            if (e < n) clashes[e] = false;
+            if (slot[at] >= 0) next[at] = atomicExch(&first[hash(slot[at])], at + 1);
+        }
+        __syncthreads();
+        constexpr int AT_ONCE = 4;
+        for (int j0 = tid; j0 < s.nseq; j0 += AT_ONCE * THREADS) {
+            int out[AT_ONCE], in[AT_ONCE];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int j = min(j0 + u * THREADS, s.nseq - 1);
+                out[u] = s.slot_out[j], in[u] = s.slot_in[j];
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; u++) {
+                const int j = min(j0 + u * THREADS, s.nseq - 1);
+                if (out[u] < 0) continue;
+                for (int e = first[hash(out[u])]; e > 0; e = next[e - 1])
+                    if (slot[e - 1] == out[u] && i0 + (e - 1) % STEP_ROWS != j) clashes[(e - 1) % STEP_ROWS] = true;
+                if (in[u] < 0) continue;
+                for (int e = first[hash(in[u])]; e > 0; e = next[e - 1])
+                    if (e <= STEP_ROWS && slot[e - 1] == in[u] && i0 + e - 1 != j) clashes[e - 1] = true;
+            }
+        }
+        __syncthreads();
+    }
+};
+
+// (At most 65535 sequences: a grid dimension.)
 inline bool step_seqs_ok(const StepSeqs& s) {
     return s.nseq >= 0 && s.nseq <= 65535 && s.rows >= 0 && s.n_slots >= 0 && (s.nseq == 0 || (s.slot_in && s.slot_out));
 }

@@ -320,6 +320,91 @@ def test_convolution_step_refuses_sequences_on_the_device(cs1, stream):
 
 # ---- paged cache ----
 
+def many_sequences(nseq, spare, hurt, seed):
+    """Windows of 0 to 3 rows; slots to begin with: the own one, none, or one of `spare` that nobody writes; who is refused."""
+    rng = np.random.default_rng(seed)
+    lens = rng.integers(0, 4, nseq)
+    start = np.concatenate([[0], np.cumsum(lens)])
+    so = rng.permutation(nseq)
+    si = np.where(rng.random(nseq) < 0.3, -1, np.where(rng.random(nseq) < 0.5, so, nseq + rng.integers(0, spare, nseq)))
+    so[rng.permutation(nseq)[:nseq // 20]] = -1                     # sit out
+    refused = np.zeros(nseq, bool)
+    if hurt:
+        some = rng.permutation(nseq)[:80]
+        so[some[:20]] = so[some[20:40]]                              # two write one slot
+        si[some[40:50]] = np.abs(so[some[50:60]])                    # one begins with what another writes
+        so[some[60:70]] = nseq + spare + rng.integers(0, 9, 10)      # no such slot
+        si[some[70:80]] = 2 ** 31 - 1
+        refused = (so >= nseq + spare) | (si >= nseq + spare)
+    outs = so[so >= 0]
+    writes, reads = (dict(zip(*np.unique(a, return_counts=True))) for a in (outs, si[(so >= 0) & (si >= 0)]))
+    for i in np.flatnonzero(so >= 0):
+        own = si[i] == so[i]
+        refused[i] |= writes[so[i]] > 1 or reads.get(so[i], 0) > own or (si[i] >= 0 and writes.get(si[i], 0) > own)
+    return lens, start, si, so, refused & (so >= 0)
+
+
+@pytest.mark.parametrize("nseq", [4095, 4096, 5003, 20003])
+@pytest.mark.parametrize("hurt", [False, True])
+def test_convolution_step_of_many_sequences(cs1, stream, nseq, hurt):
+    lens, start, si, so, refused = many_sequences(nseq, 50, hurt, nseq)
+    assert refused.any() == hurt
+    c = conv_case(start[-1], 8, 16, 2, nseq + 50, 0, nseq)
+    out, g, tails = run_conv(cs1, stream, c, start, si, so)
+    assert status()[2] in ((61, 62) if hurt else (0,))
+    y, tol, live, beta, g64, want, _ = conv_formula(c, start, si, np.where(refused, -1, so))
+    got = np.concatenate([out[m] for m in "qkv"], 1)
+    assert (got[~live] == 0x4242).all() and (out["beta"][~live] == 0x4242).all() and (g[~live] == 99.0).all()
+    assert (np.abs(f32(got) - y)[live] <= tol[live]).all()
+    assert (np.abs(f32(out["beta"]) - beta)[live] <= (HALF + 2.0 ** -20) * beta[live]).all()
+    h = np.abs(f32(c["x"])[:, c["ch"] + 2:c["ch"] + 4]) + np.abs(f32(c["dt"]))
+    assert (np.abs(g - g64)[live] <= (np.abs(g64) * (2.0 ** -20 + EPS * h))[live] + 1e-30).all()
+    assert (tails == want).all()
+
+
+@pytest.mark.parametrize("nseq", [2561, 9001])
+@pytest.mark.parametrize("hurt", [False, True])
+def test_delta_rule_step_of_many_sequences(cs1, stream, nseq, hurt):
+    H, HK, spare, scale = 4, 2, 8, D ** -0.5
+    lens, start, si, so, refused = many_sequences(nseq, spare, hurt, nseq)
+    x = delta_inputs(start[-1], H, HK, spare, nseq)
+    one = H * D * D
+    pool = L.DeviceBuffer((nseq + spare) * one * 4)                  # zeros, and the spare states at its end
+    L.check(cs1.s1_memset_async(pool.at(), 0, nseq * one * 4, stream.handle), "memset")
+    L.check(cs1.cs1_upload(pool.at(nseq * one * 4), x["states"].ctypes.data_as(C.c_void_p), x["states"].nbytes, stream.handle), "upload")
+    d = {m: up(x[m], stream) for m in ("q", "k", "v", "g", "beta")}
+    o = up(np.full(x["v"].shape, 0x4242, np.uint16), stream)
+    s, a, b = ints(start, stream), ints(si, stream), ints(so, stream)
+    L.check(cs1.s1_gdn_step(d["q"].at(), d["k"].at(), d["v"].at(), d["g"].at(), d["beta"].at(), o.at(), start[-1], H, HK, scale, pool.at(), nseq + spare,
+                            one, s.at(), a.at(), b.at(), nseq, stream.handle), "step")
+    got = down(o, x["v"].shape, stream)
+    assert status()[2] in ((61, 62) if hurt else (0,))
+    rows_of = np.repeat(np.arange(nseq), lens)
+    done = (so >= 0) & ~refused
+    assert (got[~done[rows_of]] == 0x4242).all() and (f32(got[done[rows_of]]) < 1e4).all()
+    # what no sequence leaves stays as it was
+    state = np.empty((H, D, D), np.float32)
+
+    def slot(i):
+        L.check(cs1.cs1_download(state.ctypes.data_as(C.c_void_p), pool.at(int(i) * one * 4), state.nbytes, stream.handle), "download")
+        stream.sync()
+        return state
+
+    written = set(so[done])
+    for i in [j for j in range(nseq) if j not in written][::max(1, nseq // 400)] + list(np.unique(so[refused & (so < nseq)])[:20]):
+        if i not in written:
+            assert (slot(i) == 0).all()
+    pick = np.flatnonzero(done)[::max(1, nseq // 50)]
+    rows = np.concatenate([np.arange(start[i], start[i + 1]) for i in pick])
+    part = {m: x[m][rows] for m in ("q", "k", "v", "g", "beta")}
+    part["states"] = np.concatenate([x["states"], np.zeros((len(pick), H, D, D), np.float32)])
+    at0 = np.concatenate([[0], np.cumsum(lens[pick])])
+    w, new, tol, tol_s = delta_formula(part, at0, np.where(si[pick] >= nseq, si[pick] - nseq, -1), spare + np.arange(len(pick)), H, HK, scale)
+    assert (np.abs(f32(got[rows]) - w) <= tol).all()
+    for n, i in enumerate(pick):
+        assert (np.abs(slot(so[i]) - new[spare + n]) <= tol_s[spare + n]).all()
+
+
 def make_table(need, n_pages, wide, seed):
     """Shuffled pages for sequences that need so many; -1 behind them."""
     order = np.random.default_rng(seed).permutation(n_pages)
