@@ -278,9 +278,9 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_many_kernel(cons
 //
 // Measured, in a recorded graph: 65 caches of 500 to 16000 tokens, 24 query and 4 key-value heads of 128
 // (630 MB): 103 us, 6.1 TB/s with the join; 250001 tokens, 16 and 4 heads of 256 (1.02 GB): 158 us, 6.5 TB/s;
-// 1500 tokens: 8.2 us, of which the join is 2.8; 2 tokens: 7. Before, tiles of 64 tokens of one head whose warps
-// shared every tile's maximum and probabilities: 119 us (one block per SM), 113 (two) for the first. The
-// first kernel alone takes 100 us of it: what is left is its start (2.4 us to the first tile) and the join.
+// 1500 tokens: 8.3 us; 2 tokens: 7. Without the join these are 97, 150, 5.5 and 6: the first kernel runs at the rate of a
+// copy. Before, tiles of 64 tokens of one head whose warps shared every tile's maximum and probabilities: 119 us (one
+// block per SM), 113 (two) for the first.
 constexpr int CONSUMERS = 4, PAGED_THREADS = (CONSUMERS + 1) * 32;
 constexpr int SLICE = 16;       // tokens of a warp's part of a tile, and of a copied box
 constexpr int RUN = 8, PARTS = 64;  // tiles of a run, parts of a piece: see Cut
@@ -861,8 +861,8 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
 // the parts (1500 tokens 9.0 -> 8.2 us, against notes that the first kernel left). The items are the query heads
 // of these; a warp takes one at a time, or a whole block where items are few. The order of the sums is fixed by
 // the cut alone. What follows the wait is a chain of trips to L2, so the code is kept short: unrolled further it
-// took longer to fetch than to run. (With 64 registers its blocks would fit beside running ones of the first
-// kernel, and cost that 2 us.)
+// took longer to fetch than to run. (Held to 64 registers it was 2 us slower in large calls; blocks that take 32 dims
+// of an item with four parts to a warp, so that few items keep all blocks busy, cost 1 to 4 us more.)
 constexpr int JOIN_WARPS = 16, JOIN_BLOCKS = 148;
 
 template <int DH, bool WINDOWS>
