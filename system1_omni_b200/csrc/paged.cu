@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_many_kernel(cons
 //
 // Measured, in a recorded graph: 65 caches of 500 to 16000 tokens, 24 query and 4 key-value heads of 128
 // (630 MB): 103 us, 6.1 TB/s with the join; 250001 tokens, 16 and 4 heads of 256 (1.02 GB): 158 us, 6.5 TB/s;
-// 1500 tokens: 8.3 us; 2 tokens: 7. Without the join these are 97, 150, 5.5 and 6: the first kernel runs at the rate of a
+// 1500 tokens: 8.3 us; 3 rows of 2 tokens: 8.1. Without the join: 97, 150, 5.5 and 6.5, the first kernel at the rate of a
 // copy. Before, tiles of 64 tokens of one head whose warps shared every tile's maximum and probabilities: 119 us (one
 // block per SM), 113 (two) for the first.
 constexpr int CONSUMERS = 4, PAGED_THREADS = (CONSUMERS + 1) * 32;
