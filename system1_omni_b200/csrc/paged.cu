@@ -6,8 +6,9 @@
 // p % page_tokens of page table[p / page_tokens]. Several sequences may name the same page.
 //
 // Float32 from the inputs to one rounding at the end (the prefill's operators round in between where
-// the model stores a tensor, so bf16 results may differ from theirs by a step); only the probabilities
-// are rounded to bf16 on their way into the product with the values, as in the prefill's attention.
+// the model stores a tensor, and their attention the probabilities to bf16, so bf16 results may differ from theirs
+// by a step). The probabilities go into the product with the values as two bf16 terms, off by
+// 2^-15 of their float32 values at most.
 #include <math.h>
 
 #include <algorithm>
@@ -277,8 +278,8 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_many_kernel(cons
 // float32 in the workspace, and a second kernel joins the parts of each in order.
 //
 // Measured, in a recorded graph: 65 caches of 500 to 16000 tokens, 24 query and 4 key-value heads of 128
-// (630 MB): 103 us, 6.1 TB/s with the join; 250001 tokens, 16 and 4 heads of 256 (1.02 GB): 158 us, 6.5 TB/s;
-// 1500 tokens: 8.3 us; 3 rows of 2 tokens: 8.1. Without the join: 97, 150, 5.5 and 6.5, the first kernel at the rate of a
+// (630 MB): 102 us, 6.2 TB/s with the join; 250001 tokens, 16 and 4 heads of 256 (1.02 GB): 160 us, 6.4 TB/s;
+// 1500 tokens: 8.3 us; 3 rows of 2 tokens: 7.6. Without the join: 97, 150, 5.5 and 6.5, the first kernel at the rate of a
 // copy. Before, tiles of 64 tokens of one head whose warps shared every tile's maximum and probabilities: 119 us (one
 // block per SM), 113 (two) for the first.
 constexpr int CONSUMERS = 4, PAGED_THREADS = (CONSUMERS + 1) * 32;
@@ -446,6 +447,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Two probabilities as two bf16 terms each, hi + lo within 2^-15 of p: hi is p (1 - 2^-16) cut to its upper half,
+// which lies below p wherever p > 0, so that lo > 0 too and both products with an infinite value have its sign.
+__device__ __forceinline__ void two_terms(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+    const uint32_t h0 = __float_as_uint(p0 * 0.9999847412109375f), h1 = __float_as_uint(p1 * 0.9999847412109375f);
+    hi = __byte_perm(h0, h1, 0x7632);
+    lo = pack2(p0 - __uint_as_float(h0 & 0xffff0000u), p1 - __uint_as_float(h1 & 0xffff0000u));
+}
 __device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // The warps of one head meet: all consumers, or the one warp.
@@ -469,7 +477,11 @@ __device__ __forceinline__ uint2 finish4(float4 y, float inv, bool has_gate, uin
     return make_uint2(pack2(y.x, y.y), pack2(y.z, y.w));
 }
 
-template <int DH, int HB, bool WINDOWS>
+// The second terms of the probabilities are a second product with the values (64 caches of 2000 tokens, 32 heads over one of
+// 128: 30.6 us, with one term 27.4), or with at most 8 query heads (FEW) the other 8 rows of the first: as quick as one term.
+// (Rows 8 and on of q are loaded as zeros all the same: as constants they made the compiler spill in the loop at
+// 256 dims, twice the time.)
+template <int DH, int HB, bool WINDOWS, bool FEW>
 __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
     attn_paged_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ PagedMaps maps) {
     using G = PCfg<DH>;
@@ -673,18 +685,20 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                         for (int e = 0; e < 2; e++) {
                             const int token = j * 8 + (lane & 3) * 2 + e;
                             s[j][e] = token < left_a ? (s[j][e] + s2[j][e]) * a.scale_log2 : -INFINITY;
-                            s[j][2 + e] = token < left_b ? (s[j][2 + e] + s2[j][2 + e]) * a.scale_log2 : -INFINITY;
                             xa = fmaxf(xa, s[j][e]);
-                            xb = fmaxf(xb, s[j][2 + e]);
+                            if constexpr (!FEW) {
+                                s[j][2 + e] = token < left_b ? (s[j][2 + e] + s2[j][2 + e]) * a.scale_log2 : -INFINITY;
+                                xb = fmaxf(xb, s[j][2 + e]);
+                            }
                         }
 #pragma unroll
                     for (int o = 1; o < 4; o <<= 1) {
                         xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, o));
-                        xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, o));
+                        if constexpr (!FEW) xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, o));
                     }
                     if (__any_sync(0xffffffffu, xa > ma || xb > mb)) {
                         const float na = fmaxf(ma, xa), nb = fmaxf(mb, xb);
-                        const float fa = ma == -INFINITY ? 0.f : exp2f(ma - na), fb = mb == -INFINITY ? 0.f : exp2f(mb - nb);
+                        const float fa = ma == -INFINITY ? 0.f : exp2f(ma - na), fb = FEW ? fa : mb == -INFINITY ? 0.f : exp2f(mb - nb);
                         ma = na, mb = nb;
                         la *= fa, lb *= fb;
 #pragma unroll
@@ -692,13 +706,19 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                     }
                     // a row without a finite score so far keeps offset 0: its terms are exp2(-inf) = 0
                     const float oa = ma == -INFINITY ? 0.f : ma, ob = mb == -INFINITY ? 0.f : mb;
-                    uint32_t pf[4];
+                    uint32_t pf[4], pr[4];
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        const float p0 = exp2f(s[j][0] - oa), p1 = exp2f(s[j][1] - oa), p2 = exp2f(s[j][2] - ob), p3 = exp2f(s[j][3] - ob);
-                        la += p0 + p1, lb += p2 + p3;
-                        pf[2 * j] = pack2(p0, p1);
-                        pf[2 * j + 1] = pack2(p2, p3);
+                        const float p0 = exp2f(s[j][0] - oa), p1 = exp2f(s[j][1] - oa);
+                        la += p0 + p1;
+                        if constexpr (FEW) {
+                            two_terms(p0, p1, pf[2 * j], pf[2 * j + 1]);
+                        } else {
+                            const float p2 = exp2f(s[j][2] - ob), p3 = exp2f(s[j][3] - ob);
+                            lb += p2 + p3;
+                            two_terms(p0, p1, pf[2 * j], pr[2 * j]);
+                            two_terms(p2, p3, pf[2 * j + 1], pr[2 * j + 1]);
+                        }
                     }
                     // values behind the last token may be anything, NaN included: their products with a
                     // probability of zero have to be zero
@@ -710,12 +730,21 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                         uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
                         if (left < SLICE) keep[0] = kept(left, 0), keep[1] = kept(left, 1);
 #pragma unroll
-                        for (int t = 0; t < NT; t += 2) {
-                            const int ch = v_ch + t;
-                            uint32_t b[4];
-                            ldsm4_t(b, vb + (ch >> 3) * (SLICE * 128) + v_tok * 128 + (((ch ^ v_tok) & 7) << 4));
-                            mma16816(acc[t], pf, b[0] & keep[0], b[1] & keep[1]);
-                            mma16816(acc[t + 1], pf, b[2] & keep[0], b[3] & keep[1]);
+                        for (int t = 0; t < NT; t += 4) {
+                            uint32_t b[2][4];
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const int ch = v_ch + t + 2 * u;
+                                ldsm4_t(b[u], vb + (ch >> 3) * (SLICE * 128) + v_tok * 128 + (((ch ^ v_tok) & 7) << 4));
+#pragma unroll
+                                for (int e = 0; e < 4; e++) b[u][e] &= keep[e & 1];
+                            }
+#pragma unroll
+                            for (int u = 0; u < 4; u++) mma16816(acc[t + u], pf, b[u / 2][u % 2 * 2], b[u / 2][u % 2 * 2 + 1]);
+                            if constexpr (!FEW) {
+#pragma unroll
+                                for (int u = 0; u < 4; u++) mma16816(acc[t + u], pr, b[u / 2][u % 2 * 2], b[u / 2][u % 2 * 2 + 1]);
+                            }
                         }
                     } else {
                         // a token that one row of the window has and another has not: each row on its own
@@ -726,6 +755,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                             const bool is_a = of_window(ra) == i, is_b = of_window(rb) == i;
                             const uint32_t keep[2] = {kept(tokens, 0), kept(tokens, 1)};
                             const uint32_t own[4] = {is_a ? pf[0] : 0, is_b ? pf[1] : 0, is_a ? pf[2] : 0, is_b ? pf[3] : 0};
+                            const uint32_t rest[4] = {is_a ? pr[0] : 0, is_b ? pr[1] : 0, is_a ? pr[2] : 0, is_b ? pr[3] : 0};
 #pragma unroll
                             for (int t = 0; t < NT; t += 2) {
                                 const int ch = v_ch + t;
@@ -734,6 +764,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
 #pragma unroll
                                 for (int u = 0; u < 2; u++) {
                                     float x[4] = {acc[t + u][0], acc[t + u][1], acc[t + u][2], acc[t + u][3]};
+                                    mma16816(x, rest, b[2 * u] & keep[0], b[2 * u + 1] & keep[1]);
                                     mma16816(x, own, b[2 * u] & keep[0], b[2 * u + 1] & keep[1]);
                                     if (is_a) acc[t + u][0] = x[0], acc[t + u][1] = x[1];
                                     if (is_b) acc[t + u][2] = x[2], acc[t + u][3] = x[3];
@@ -747,6 +778,10 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
             }
 
             // ---- the piece's end ----
+            if constexpr (FEW) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[t][0] += acc[t][2], acc[t][1] += acc[t][3];
+            }
             // The warps hand their weighted values over in shared memory, some dims at a time, and those of a head
             // sum, norm and write them. One loop for it, the accumulators moving up: unrolled, the code took longer to
             // fetch than to run, and every gate waited for the store before it (5 us a piece at 128 dims, 17 at 256).
@@ -820,7 +855,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
                 for (int t = 0; t < G::PART / 8; t++) {
                     const int d = t * 8 + (lane & 3) * 2;
                     *reinterpret_cast<float2*>(box + ra * G::PITCH + d) = make_float2(acc[t][0] * fa, acc[t][1] * fa);
-                    *reinterpret_cast<float2*>(box + rb * G::PITCH + d) = make_float2(acc[t][2] * fb, acc[t][3] * fb);
+                    if constexpr (!FEW) *reinterpret_cast<float2*>(box + rb * G::PITCH + d) = make_float2(acc[t][2] * fb, acc[t][3] * fb);
                 }
                 piece_sync<SUBS>();
 #pragma unroll
@@ -1065,27 +1100,27 @@ bool table_ok(const PageTable& t) {
 // Key-value heads of a tile: as many as share the pool's rows, up to a warp each.
 inline int head_block(int Hk) { return Hk % 4 == 0 ? 4 : Hk % 2 == 0 ? 2 : 1; }
 
-template <int DH, int HB, bool WINDOWS>
+template <int DH, int HB, bool WINDOWS, bool FEW>
 int run_paged(const PagedArgs& a, const PagedMaps& maps, int dev, int blocks, cudaStream_t st) {
     using G = PCfg<DH>;
     static bool configured[64] = {};
     if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_paged_kernel<DH, HB, WINDOWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(attn_paged_kernel<DH, HB, WINDOWS, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
         if (e != cudaSuccess) return e;
         configured[dev] = true;
     }
-    cudaError_t e = launch_dep_family(DEP_ATTENTION, attn_paged_kernel<DH, HB, WINDOWS>, blocks, PAGED_THREADS, G::SMEM, st, a, maps);
+    cudaError_t e = launch_dep_family(DEP_ATTENTION, attn_paged_kernel<DH, HB, WINDOWS, FEW>, blocks, PAGED_THREADS, G::SMEM, st, a, maps);
     if (e != cudaSuccess) return e;
     // always a programmatic dependent: it waits for the first kernel before it reads anything of it
     e = launch_maybe_dep(true, attn_paged_join_kernel<DH, WINDOWS>, JOIN_BLOCKS, JOIN_WARPS * 32, 0, st, a, blocks, HB);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <int DH, bool WINDOWS>
+template <int DH, bool WINDOWS, bool FEW>
 int run_paged(int HB, const PagedArgs& a, const PagedMaps& maps, int dev, int blocks, cudaStream_t st) {
-    return HB == 4   ? run_paged<DH, 4, WINDOWS>(a, maps, dev, blocks, st)
-           : HB == 2 ? run_paged<DH, 2, WINDOWS>(a, maps, dev, blocks, st)
-                     : run_paged<DH, 1, WINDOWS>(a, maps, dev, blocks, st);
+    return HB == 4   ? run_paged<DH, 4, WINDOWS, FEW>(a, maps, dev, blocks, st)
+           : HB == 2 ? run_paged<DH, 2, WINDOWS, FEW>(a, maps, dev, blocks, st)
+                     : run_paged<DH, 1, WINDOWS, FEW>(a, maps, dev, blocks, st);
 }
 
 // Blocks of a call at most: what its workspace is for.
@@ -1197,6 +1232,10 @@ extern "C" int s1_attention_paged(const void* q, const void* gate, void* out, co
     const double bytes = (double)n_seqs * table_pages * page_tokens * Hk * Dh * 4;
     const bool windows = seq && rows > n_seqs && rows <= WINDOW_ROWS && bytes * (a.window - 1) >= 64e6;
     if (windows)
-        return Dh == 256 ? run_paged<256, true>(HB, a, maps, dev, blocks, st) : run_paged<128, true>(HB, a, maps, dev, blocks, st);
-    return Dh == 256 ? run_paged<256, false>(HB, a, maps, dev, blocks, st) : run_paged<128, false>(HB, a, maps, dev, blocks, st);
+        return Dh == 256 ? run_paged<256, true, false>(HB, a, maps, dev, blocks, st) : run_paged<128, true, false>(HB, a, maps, dev, blocks, st);
+    // Few heads, the second terms in the idle rows against a second product: 8000 tokens of 24 and 4 heads 12.3 us and 14.4, 32 x
+    // 32,000 313 and 325, 250001 tokens of 16 and 4 heads of 256, called for seconds on end, 162 and 167.
+    if (a.chunk <= 8)
+        return Dh == 256 ? run_paged<256, false, true>(HB, a, maps, dev, blocks, st) : run_paged<128, false, true>(HB, a, maps, dev, blocks, st);
+    return Dh == 256 ? run_paged<256, false, false>(HB, a, maps, dev, blocks, st) : run_paged<128, false, false>(HB, a, maps, dev, blocks, st);
 }

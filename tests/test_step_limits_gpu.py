@@ -1,0 +1,92 @@
+"""The decode operators on the GPU where their promises are tightest: the probabilities' precision, infinite values,
+codes next to a prefill, grouped calls at their limits."""
+import numpy as np
+import pytest
+
+import test_step_gpu as S
+from helpers import bf, f32
+from system1_omni_b200 import lib as L
+
+pytestmark = pytest.mark.gpu
+
+HALF, EPS, NAN = S.HALF, S.EPS, S.NAN
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cs1, stream):
+    S.status()
+    yield
+    assert S.status() == (0, 0, 0)
+
+
+# ---- attention: the precision of the probabilities ----
+
+def exact_scores(c, seed):
+    """The case with queries and keys whose scores float32 holds exactly: four dims of quarters up to 2."""
+    rng = np.random.default_rng(seed)
+    quarters = lambda shape: bf(rng.integers(-8, 9, shape) * 0.25 * (np.arange(shape[-1]) < 4))
+    return dict(c, q=quarters(c["q"].shape), kp=np.where(c["kp"] == NAN, NAN, quarters(c["kp"].shape)))
+
+
+def tight_formula(c, r, gated):
+    """Result and bound with exact scores s, |s| <= 16, scale 1 and up to 64 tokens. Of p: 2^-15 from its two bf16 terms;
+    s log2(e) up to 24 and rounded twice (constant and product), as the maximum is, then their difference rounded:
+    ln 2 * (4 * 24 + 48) * 2^-24 < 2^-17; exp2f 2^-22. Sums of p over at most 4 slices of 16 tokens, 2^-24 an addition:
+    24 additions, 2^-19. The product: 8 MMAs of 16 terms and what came before, 17 * 2^-24 each, 2^-16.9. Rescaling
+    and the division, 2^-21. Together below 2^-14."""
+    want, _ = S.attn_formula(c, r, False, 1.0)
+    n = c["lens"][r]
+    _, size = np.abs(want), S.attn_formula(dict(c, vp=c["vp"] & np.uint16(0x7fff)), r, False, 1.0)[0]   # sum of p |v|
+    assert n <= 64
+    if gated:
+        w = 1 / (1 + np.exp(-f32(c["gate"][r]).astype(np.float64)))
+        want, size = want * w, size * w
+    # the gate: __expf 2^-21 relative to its argument's size and __fdividef 2^-22, together below 2^-18
+    return want, (2.0 ** -14 + (2.0 ** -18 if gated else 0)) * size + HALF * np.abs(want) * (1 + 2.0 ** -13)
+
+
+@pytest.mark.parametrize("Dh", [128, 256])
+@pytest.mark.parametrize("Hq,Hk,page", [(24, 4, 64), (8, 8, 16), (6, 2, 16), (16, 2, 32), (5, 1, 16), (32, 1, 16)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_probabilities_enter_the_product_as_float32(cs1, stream, Dh, Hq, Hk, page, gated):
+    c = exact_scores(S.attn_case([2, 64, 17, 33, 48, 3, 63, 1, 9, 40], Hq, Hk, Dh, page, Hq + Dh), 5)
+    got = S.run_attn(cs1, stream, c, gated, 1.0)
+    for r in range(len(c["lens"])):
+        want, tol = tight_formula(c, r, gated)
+        err = np.abs(f32(got[r]).astype(np.float64) - want)
+        assert (err <= tol).all(), (r, (err / tol).max())
+
+
+@pytest.mark.parametrize("Dh,Hq,Hk", [(128, 16, 4), (128, 24, 4), (128, 8, 8), (256, 6, 2), (256, 16, 4), (128, 5, 1)])
+def test_probabilities_of_a_window_enter_the_product_as_float32(cs1, stream, Dh, Hq, Hk):
+    lens, seq = S.windows_of([(0, 30, 3, 1), (1, 60, 5, 1), (2, 9, 4, 5)])     # over the ends of slices and within them
+    c = S.wide(exact_scores(S.attn_case(lens, Hq, Hk, Dh, 16, Hq + Dh, seq=seq), 6))
+    got = S.run_attn(cs1, stream, c, False, 1.0)
+    for r in range(len(lens)):
+        want, tol = tight_formula(c, r, False)
+        err = np.abs(f32(got[r]).astype(np.float64) - want)
+        assert (err <= tol).all(), (r, (err / tol).max())
+
+
+@pytest.mark.parametrize("Dh,Hq,Hk", [(128, 8, 4), (256, 8, 2), (128, 5, 1)])
+@pytest.mark.parametrize("equal", [True, False])
+@pytest.mark.parametrize("window", [True, False])
+def test_infinite_values_keep_their_sign(cs1, stream, Dh, Hq, Hk, equal, window):
+    """An infinite value of a token that a row sees makes that dim infinite, whatever the token's weight, and no other dim."""
+    lens, seq = S.windows_of([(0, 40, 4, 1), (1, 1, 1, 0), (2, 100, 3, 1)])
+    c = S.attn_case(lens, Hq, Hk, Dh, 16, 8, seq=seq)
+    if equal:
+        c["q"] = c["q"] * np.uint16(0)
+    if window:
+        c = S.wide(c)
+    finite = [S.attn_formula(c, r, False, Dh ** -0.5) for r in range(len(lens))]
+    for s, t, d, bits in [(0, 0, 3, 0x7f80), (0, 39, 70, 0xff80), (1, 0, 9, 0x7f80), (2, 57, 127, 0xff80)]:
+        c["vp"][c["table"][s, t // 16], t % 16, :, d] = bits
+    got = f32(S.run_attn(cs1, stream, c, False, Dh ** -0.5))
+    for r, s in enumerate(seq):
+        hit = {0: {3: np.inf, 70: -np.inf}, 1: {9: np.inf}, 2: {127: -np.inf}}[s]
+        for d, x in hit.items():
+            assert (got[r, :, d] == x).all(), (r, d)
+        rest = [d for d in range(Dh) if d not in hit]
+        want, tol = finite[r]
+        assert (np.abs(got[r][:, rest] - want[:, rest]) <= tol[:, rest]).all()
