@@ -71,12 +71,23 @@ def build_compare():
 
 
 def build_fastcall():
-    """The direct binding of the step operators (a CPython extension; lib.py uses ctypes where it is absent)."""
+    """The direct binding of the step operators, a CPython extension for the interpreter that builds it. Without Python's
+    headers there is none (None is returned), and lib.py calls through ctypes."""
     src = os.path.join(PKG, "binding", "fastcall.cpp")
-    out = os.path.join(PKG, "_fastcall.so")
-    if _stale(out, [src, os.path.join(ROOT, "include", "s1_executor.h")]):
-        subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-I" + sysconfig.get_paths()["include"],
-                        "-I" + os.path.join(ROOT, "include"), "-o", out, src], check=True)
+    out = os.path.join(PKG, "_fastcall" + sysconfig.get_config_var("EXT_SUFFIX"))
+    untagged = os.path.join(PKG, "_fastcall.so")  # an earlier build's name, which any interpreter would load
+    if os.path.exists(untagged):
+        os.remove(untagged)
+    if not _stale(out, [src, os.path.join(ROOT, "include", "s1_executor.h")]):
+        return out
+    include = sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(include, "Python.h")):
+        sys.stderr.write(f"{include} has no Python.h: the step operators are called through ctypes\n")
+        if os.path.exists(out):
+            os.remove(out)  # it may know other prototypes
+        return None
+    subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-shared", "-fPIC", "-I" + include, "-I" + os.path.join(ROOT, "include"),
+                    "-o", out, src], check=True)
     return out
 
 
