@@ -23,7 +23,7 @@
 /* Library-defined error codes (>= 1000, as src/backends/cuda/contract.md:145-148 reserves). */
 #define CS1_ERR_GEMM_BASE 1000      /* 1000 + cublasStatus_t, as the reference (gemm.cu:34) */
 #define CS1_ERR_UNSUPPORTED 2000    /* this engine does not take the problem (see s1_gemm_swiglu, s1_gemm_tcgen05) */
-#define CS1_ERR_DEVICE_CHECK 2001   /* a device-side bounded wait gave up, or a step operator refused an index */
+#define CS1_ERR_DEVICE_CHECK 2001   /* a device-side bounded wait gave up */
 #define CS1_ERR_TENSOR_MAP 2002     /* a TMA tensor map could not be encoded */
 #define CS1_ERR_STATIC_SCRATCH 2003 /* the window does not fit the fixed scratch of cs1_gdn_prefill_static */
 

@@ -103,11 +103,12 @@ int s1_gdn_conv_gates_batch(const void* qkv, int ld, const void* w, void* q, voi
  * results differ from theirs by a step of bf16 at times). Everything that changes from step to step
  * (slots, positions, lengths, page tables) is int32 in device memory, so a recorded step replays with
  * new contents; the kernels check every index before they use it. What they refuse they leave
- * unwritten, with a code in the family's device error word (s1_device_status): 60 rows outside the
+ * unwritten, with a code in a device error word of the family's step operators: 60 rows outside the
  * operands, 61 a slot outside the pool, 62 sequences that would race for a slot (delta-rule family);
  * 31 a row whose sequence or position the table does not have, 32 a page outside the pools, 33 a
  * position outside the rotary tables, 34 rows at one place of the cache, 30 a bounded wait that ran out
- * (attention family). A code stays until it is read, and the executor's calls that check the words report it too.
+ * (attention family). A code stays until s1_device_status, s1_gdn_status or s1_attn_tc5_status reads it; the
+ * executor's calls neither report nor clear it, so an index that one host thread gets wrong fails no other's prefill.
  * The first call of an operator on a GPU looks up the address of that word: make it before any
  * stream capture. All pointers belong to the current device, as everywhere in this interface. */
 
@@ -207,9 +208,10 @@ int s1_attn_tc5_status(int* code);
 
 /* The same for the delta-rule kernels (a bounded wait for a TMA or bulk copy gave up). */
 int s1_gdn_status(int* code);
-/* All three words of the current device with one wait for the device (each out pointer nullable);
- * cleared when any is set. The executor's calls that read results back (s1_model_forward_batch,
- * s1_model_forward_continue, s1_model_prefix_capture, s1_model_read_rows) check them themselves
+/* All words of the current device with one wait for the device (each out pointer nullable), cleared as they
+ * are reported. attention and gdn carry the step operators' codes (30-34, 60-62) too, where no kernel of a prefill has
+ * left one. The executor's calls that read results back (s1_model_forward_batch,
+ * s1_model_forward_continue, s1_model_prefix_capture, s1_model_read_rows) check the prefill's words themselves
  * and return CS1_ERR_DEVICE_CHECK, the way the reference turns every device failure into an
  * error (src/models/qwen3_5/native/src/cuda.rs:177-187). */
 int s1_device_status(int* gemm, int* attention, int* gdn);

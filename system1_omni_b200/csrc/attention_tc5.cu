@@ -553,7 +553,7 @@ int s1_attn_tc5_full64(const bf16* q, const bf16* k, const bf16* v, int ldv, bf1
 }
 
 // The device error word of the attention kernel on the current device (0 = no bounded wait ever
-// gave up) after waiting for all queued work; cleared by the call.
+// gave up) after waiting for all queued work, or else the code of the step operators; cleared by the call.
 extern "C" int s1_attn_tc5_status(int* code) {
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return e;
@@ -563,6 +563,8 @@ extern "C" int s1_attn_tc5_status(int* code) {
     if (v != 0) {
         const int zero = 0;
         e = cudaMemcpyToSymbol(g_attn_error, &zero, sizeof(int));
+    } else {
+        e = (cudaError_t)s1::take_step_error(s1::STEP_ATTENTION, &v);
     }
     *code = v;
     return e;

@@ -884,7 +884,7 @@ int gdn_run(const void* q, const void* k, const void* v, const float* g, const v
 using namespace s1;
 
 // The device error word of the delta-rule kernels on the current device (0 = no bounded wait
-// ever gave up) after waiting for all queued work; cleared by the call.
+// ever gave up) after waiting for all queued work, or else the code of the step operators; cleared by the call.
 extern "C" int s1_gdn_status(int* code) {
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return e;
@@ -894,6 +894,8 @@ extern "C" int s1_gdn_status(int* code) {
     if (v != 0) {
         const int zero = 0;
         e = cudaMemcpyToSymbol(s1::g_gdn_error, &zero, sizeof(int));
+    } else {
+        e = (cudaError_t)s1::take_step_error(s1::STEP_GDN, &v);
     }
     *code = v;
     return e;

@@ -56,7 +56,43 @@ __global__ void collect_status_kernel(const int* a, const int* b, const int* c, 
     out[2] = *c;
 }
 
+__device__ int g_step_error[2];  // by StepFamily
+
+// Reads a word, and clears it if it is set.
+cudaError_t take_word(int* word, int* code) {
+    cudaError_t e = cudaMemcpy(code, word, sizeof(int), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && *code != 0) e = cudaMemset(word, 0, sizeof(int));
+    return e;
+}
+
 }  // namespace
+
+int step_error_address(StepFamily family, int** p) {
+    void* a = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&a, g_step_error);
+    *p = static_cast<int*>(a) + family;
+    return e;
+}
+
+int take_step_error(StepFamily family, int* code) {
+    int* word = nullptr;
+    const cudaError_t e = (cudaError_t)step_error_address(family, &word);
+    return e != cudaSuccess ? e : take_word(word, code);
+}
+
+static int device_status(int (&v)[3]) {
+    int* p[3] = {};
+    cudaError_t e;
+    if ((e = (cudaError_t)gemm_error_address(&p[0])) != cudaSuccess) return e;
+    if ((e = (cudaError_t)attn_error_address(&p[1])) != cudaSuccess) return e;
+    if ((e = (cudaError_t)gdn_error_address(&p[2])) != cudaSuccess) return e;
+    if ((e = cudaDeviceSynchronize()) != cudaSuccess) return e;
+    for (int i = 0; i < 3; i++)
+        if ((e = take_word(p[i], &v[i])) != cudaSuccess) return e;
+    if (v[1] == 0 && (e = (cudaError_t)take_step_error(STEP_ATTENTION, &v[1])) != cudaSuccess) return e;
+    if (v[2] == 0 && (e = (cudaError_t)take_step_error(STEP_GDN, &v[2])) != cudaSuccess) return e;
+    return cudaSuccess;
+}
 
 int collect_status(int* out3_device, cudaStream_t st) {
     int *a = nullptr, *b = nullptr, *c = nullptr;
@@ -104,22 +140,12 @@ int spread_block(void* dst, size_t row_packs, const int* row0, int n, const void
 
 }  // namespace s1
 
-// The three device error words of the current device after waiting for all queued work
-// (0 = no bounded wait gave up), cleared when any is set. Every out pointer is nullable.
+// The device error words of the current device after waiting for all queued work (0 = no bounded wait gave up and
+// no step operator refused an index), those that are reported cleared. Every out pointer is nullable.
 extern "C" int s1_device_status(int* gemm, int* attention, int* gdn) {
-    int* p[3] = {};
-    cudaError_t e;
-    if ((e = (cudaError_t)s1::gemm_error_address(&p[0])) != cudaSuccess) return e;
-    if ((e = (cudaError_t)s1::attn_error_address(&p[1])) != cudaSuccess) return e;
-    if ((e = (cudaError_t)s1::gdn_error_address(&p[2])) != cudaSuccess) return e;
-    if ((e = cudaDeviceSynchronize()) != cudaSuccess) return e;
     int v[3] = {};
-    for (int i = 0; i < 3; i++)
-        if ((e = cudaMemcpy(&v[i], p[i], sizeof(int), cudaMemcpyDeviceToHost)) != cudaSuccess) return e;
-    if (v[0] | v[1] | v[2]) {
-        const int rc = s1::clear_status();
-        if (rc != 0) return rc;
-    }
+    const int rc = s1::device_status(v);
+    if (rc != 0) return rc;
     if (gemm) *gemm = v[0];
     if (attention) *attention = v[1];
     if (gdn) *gdn = v[2];

@@ -25,7 +25,7 @@ namespace {
 
 using namespace tc5;
 
-// Codes left in the attention family's device error word.
+// Codes left in the attention step operators' device error word.
 enum { PAGED_WAIT = 30, PAGED_BAD_ROW = 31, PAGED_BAD_PAGE = 32, PAGED_BAD_ANGLE = 33, PAGED_CLASH = 34 };
 
 struct PageTable {
@@ -1076,7 +1076,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) attn_paged_join_kernel(const 
     }
 }
 
-// The attention family's error word on the current device, looked up once per device.
+// The attention step operators' error word on the current device, looked up once per device.
 int error_word(int** p, int* device) {
     static int* address[64] = {};
     const cudaError_t e = cudaGetDevice(device);
@@ -1084,7 +1084,7 @@ int error_word(int** p, int* device) {
     if (*device >= 64) return cudaErrorInvalidDevice;
     if (!address[*device]) {
         int* a = nullptr;
-        const int rc = attn_error_address(&a);
+        const int rc = step_error_address(STEP_ATTENTION, &a);
         if (rc != 0) return rc;
         address[*device] = a;
     }

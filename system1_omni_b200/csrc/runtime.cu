@@ -15,7 +15,7 @@ const char* cs1_error_string(int code) {
     if (code >= CS1_ERR_GEMM_BASE && code < CS1_ERR_UNSUPPORTED) return "GEMM handle or engine error (code - 1000)";
     switch (code) {
         case CS1_ERR_UNSUPPORTED: return "operation not built into this library";
-        case CS1_ERR_DEVICE_CHECK: return "a device-side bounded wait gave up, or a step operator refused an index";
+        case CS1_ERR_DEVICE_CHECK: return "a device-side bounded wait gave up";
         case CS1_ERR_TENSOR_MAP: return "TMA tensor map encoding failed";
         case CS1_ERR_STATIC_SCRATCH: return "window larger than the fixed scratch of cs1_gdn_prefill_static";
         case 3000: return "executor: invalid argument";

@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(CONV_THREADS)
     } while (MANY && ++i < min(i0 + per, seqs.nseq));
 }
 
-// The delta-rule family's error word on the current device, looked up once per device.
+// The delta-rule step operators' error word on the current device, looked up once per device.
 int error_word(int** p) {
     static int* address[64] = {};
     int dev = 0;
@@ -339,7 +339,7 @@ int error_word(int** p) {
     if (dev >= 64) return cudaErrorInvalidDevice;
     if (!address[dev]) {
         int* a = nullptr;
-        const int rc = gdn_error_address(&a);
+        const int rc = step_error_address(STEP_GDN, &a);
         if (rc != 0) return rc;
         address[dev] = a;
     }

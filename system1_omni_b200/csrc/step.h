@@ -12,7 +12,7 @@ struct StepSeqs {
     int nseq, rows, n_slots;
 };
 
-// Codes that the step operators leave in a family's device error word.
+// Codes that the delta-rule step operators leave in their device error word.
 enum { STEP_BAD_ROWS = 60, STEP_BAD_SLOT = 61, STEP_SLOT_CLASH = 62 };
 
 struct StepSeq {

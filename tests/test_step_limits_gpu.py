@@ -90,3 +90,53 @@ def test_infinite_values_keep_their_sign(cs1, stream, Dh, Hq, Hk, equal, window)
         rest = [d for d in range(Dh) if d not in hit]
         want, tol = finite[r]
         assert (np.abs(got[r][:, rest] - want[:, rest]) <= tol[:, rest]).all()
+
+
+# ---- codes next to a prefill ----
+
+@pytest.fixture(scope="module")
+def model(cs1):
+    from helpers import random_weights, tiny_config
+    from system1_omni_b200 import model as M
+    L.set_device(0)
+    cfg = tiny_config()
+    m = M.Model(cfg, device=0)
+    m.set_tensors(random_weights(cfg, seed=4))
+    yield m
+    m.close()
+
+
+@pytest.mark.parametrize("family", ["delta rule", "convolution", "prep", "attention"])
+def test_a_refused_index_fails_no_prefill(cs1, stream, model, family):
+    """A step operator's refusal is its caller's: a pass of the executor behind it gives its rows, and the code is still there."""
+    prompts = [list(range(1, 50)), list(range(7, 300))]
+    before = model.forward_batch(prompts)
+    if family == "delta rule":
+        x = S.delta_inputs(2, 2, 1, 3, 1)
+        S.run_delta(cs1, stream, x, None, np.array([0, 9]), np.array([0, 1]), 2, 1, 1.0)
+        want = (0, 0, 61)
+    elif family == "convolution":
+        S.run_conv(cs1, stream, S.conv_case(2, 128, 128, 1, 3, 0, 1), None, np.array([0, 1]), np.array([1, 1]))
+        want = (0, 0, 62)
+    elif family == "prep":
+        p = S.prep_inputs(2, 2, 1, 128, 32, 50, 4, 16, 0, 1)
+        S.run_prep(cs1, stream, p, np.array([[0, 1], [2, 9]], np.int32), [0, 1], [3, 20])
+        want = (0, 32, 0)
+    else:
+        c = S.attn_case([20, 30], 2, 1, 128, 16, 1)
+        S.run_attn(cs1, stream, dict(c, seq=[0, 5]), False, 1.0)
+        want = (0, 31, 0)
+    stream.sync()
+    assert (model.forward_batch(prompts) == before).all()
+    assert (model.forward_batch(prompts) == before).all()
+    assert S.status() == want
+
+
+@pytest.mark.parametrize("read,want", [("attn_status", 31), ("gdn_status", 61)])
+def test_the_families_status_calls_report_the_steps_codes(cs1, stream, read, want):
+    c = S.attn_case([20, 30], 2, 1, 128, 16, 1)
+    S.run_attn(cs1, stream, dict(c, seq=[0, 5]), False, 1.0)
+    S.run_delta(cs1, stream, S.delta_inputs(2, 2, 1, 3, 1), None, np.array([0, 9]), np.array([0, 1]), 2, 1, 1.0)
+    assert getattr(L, read)() == want
+    assert getattr(L, read)() == 0
+    assert S.status() == ((0, 0, 61) if read == "attn_status" else (0, 31, 0))     # the other family's stays until it is read
