@@ -131,7 +131,7 @@ __device__ __forceinline__ void softmax_rows(unsigned char* smem, uint64_t* bars
     for (int j = 0; j < ntiles; j++) {
         const int b = j & 1;
         if (ok && !mbar_wait(&s_full[b], (j >> 1) & 1, abort_flag)) {
-            fail(31);
+            fail(35);
             ok = false;
         }
         uint32_t sv[HN];
@@ -185,7 +185,7 @@ __device__ __forceinline__ void softmax_rows(unsigned char* smem, uint64_t* bars
         if (j > 0) {
             // P V of the previous tile is complete: the accumulator may be rescaled and P overwritten
             if (!mbar_wait(o_done, (j - 1) & 1, abort_flag)) {
-                fail(32);
+                fail(36);
                 ok = false;
                 continue;
             }
@@ -227,7 +227,7 @@ __device__ __forceinline__ void softmax_rows(unsigned char* smem, uint64_t* bars
     asm volatile("bar.sync 1, 256;" ::: "memory");
     if (!ok || ntiles == 0) return;
     if (!mbar_wait(o_done, (ntiles - 1) & 1, abort_flag)) {
-        fail(33);
+        fail(37);
         return;
     }
     fence_after_sync();

@@ -314,3 +314,16 @@ def test_direct_calls_answer_as_ctypes_does(cs1):
     wide[16] = 1 << 32                                                  # ctypes keeps the low 32 bits of an int: nseq 0
     assert f(*wide) == 0
     assert f(*plain[:6], True, *plain[7:]) == 0
+
+
+def test_an_error_code_names_one_thing():
+    """s1_device_status reports a family's waits and its step operators' refusals in one place: no code stands for both."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "system1_omni_b200", "csrc")
+    read = lambda name: open(os.path.join(csrc, name)).read()
+    for waits, steps, enum in (("attention_tc5.cu", "paged.cu", r"PAGED_\w+ = (\d+)"), ("gdn.cu", "step.h", r"STEP_[A-Z_]+ = (\d+)")):
+        of_waits = set(re.findall(r"fail\((\d+)\)", read(waits))) | set(re.findall(r"atomicCAS\(&\w+, 0, (\d+)\)", read(waits)))
+        of_steps = set(re.findall(enum, read(steps)))
+        assert of_waits and len(of_steps) >= 3
+        assert not of_waits & of_steps
