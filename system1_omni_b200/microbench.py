@@ -150,9 +150,9 @@ def step(b, out):
     for op, layers, nbytes in (("fork_states", 48, H * 128 * 128 * 4), ("fork_pages", 32, page * Hk * Dh * 2)):
         pools = [L.DeviceBuffer(9 * nbytes) for _ in range(layers)]
         ptrs = (C.c_void_p * layers)(*[p.ptr.value for p in pools])
-        a, d = np.zeros(8, np.int32), np.arange(1, 9, dtype=np.int32)
-        src, dst = a.ctypes.data, d.ctypes.data
-        us = b.time(lambda i: lib.s1_pages_copy(C.addressof(ptrs), layers, 9, nbytes, src, dst, 8, st), 1)
+        first, rest = np.zeros(8, np.int32), np.arange(1, 9, dtype=np.int32)
+        at_first, at_rest, at_pools = first.ctypes.data, rest.ctypes.data, C.addressof(ptrs)
+        us = b.time(lambda i: lib.s1_pages_copy(at_pools, layers, 9, nbytes, at_first, at_rest, 8, st), 1)
         report(op, 8, None, 9 * layers * nbytes, us)
         del pools
 
