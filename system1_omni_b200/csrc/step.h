@@ -48,23 +48,41 @@ __device__ __forceinline__ bool step_clash(const StepSeqs& s, int i, int in, int
 }
 
 // The same for `n` sequences of a block, i0 and on, at once: every other sequence's slots are looked up among theirs,
-// which for many sequences takes a fraction of comparing all with all in every block. All threads of the block call it.
+// which for many sequences takes a fraction of comparing all with all in every block. What they write and what they
+// begin with are looked up apart: sequences may share a slot to begin with, and all of a block that do are one chain, in which
+// only slots that someone writes are looked up; a bit of another hash keeps those off it that merely fall into its place.
+// A chain of slots to write is short, or its sequences are refused. All threads of the block call it.
 constexpr int STEP_ROWS = 128;
 struct StepLookup {
     static constexpr int HASH = 512;
-    int first[HASH], next[2 * STEP_ROWS], slot[2 * STEP_ROWS];  // chains of 1 + entry; entries: outs, then ins
+    struct Slots {
+        int first[HASH], next[STEP_ROWS], slot[STEP_ROWS];  // chains of 1 + entry
+        uint32_t bits[HASH];                                // of the slots in a chain
+        __device__ __forceinline__ void put(int e, int s) {
+            slot[e] = s;
+            if (s < 0) return;
+            next[e] = atomicExch(&first[hash(s)], e + 1);
+            atomicOr(&bits[hash(s)], bit(s));
+        }
+    } outs, ins;
     bool clashes[STEP_ROWS];
     static __device__ __forceinline__ uint32_t hash(int s) { return (uint32_t)s * 2654435769u >> 23; }
+    static __device__ __forceinline__ uint32_t bit(int s) { return 1u << ((uint32_t)s * 2654435769u >> 18 & 31); }
+    // Marks the block's sequences that have slot s in `of`, but for `own`, the one that it is looked up for.
+    __device__ __forceinline__ void mark(const Slots& of, int s, int own) {
+        if (!(of.bits[hash(s)] & bit(s))) return;
+        for (int e = of.first[hash(s)]; e > 0; e = of.next[e - 1])
+            if (of.slot[e - 1] == s && e - 1 != own) clashes[e - 1] = true;
+    }
     template <int THREADS>
     __device__ __forceinline__ void find(const StepSeqs& s, int i0, int n) {
         const int tid = threadIdx.x;
-        for (int e = tid; e < HASH; e += THREADS) first[e] = 0;
+        for (int e = tid; e < HASH; e += THREADS) outs.first[e] = ins.first[e] = 0, outs.bits[e] = ins.bits[e] = 0;
         __syncthreads();
-        for (int e = tid; e < 2 * n; e += THREADS) {
-            const int at = e < n ? e : STEP_ROWS + e - n;
-            slot[at] = e < n ? s.slot_out[i0 + e] : s.slot_in[i0 + e - n];
-            if (e < n) clashes[e] = false;
-            if (slot[at] >= 0) next[at] = atomicExch(&first[hash(slot[at])], at + 1);
+        for (int e = tid; e < n; e += THREADS) {
+            clashes[e] = false;
+            outs.put(e, s.slot_out[i0 + e]);
+            ins.put(e, s.slot_in[i0 + e]);
         }
         __syncthreads();
         constexpr int AT_ONCE = 4;
@@ -77,13 +95,11 @@ struct StepLookup {
             }
 #pragma unroll
             for (int u = 0; u < AT_ONCE; u++) {
-                const int j = min(j0 + u * THREADS, s.nseq - 1);
+                const int own = min(j0 + u * THREADS, s.nseq - 1) - i0;
                 if (out[u] < 0) continue;
-                for (int e = first[hash(out[u])]; e > 0; e = next[e - 1])
-                    if (slot[e - 1] == out[u] && i0 + (e - 1) % STEP_ROWS != j) clashes[(e - 1) % STEP_ROWS] = true;
-                if (in[u] < 0) continue;
-                for (int e = first[hash(in[u])]; e > 0; e = next[e - 1])
-                    if (e <= STEP_ROWS && slot[e - 1] == in[u] && i0 + e - 1 != j) clashes[e - 1] = true;
+                mark(outs, out[u], own);
+                mark(ins, out[u], own);
+                if (in[u] >= 0) mark(outs, in[u], own);
             }
         }
         __syncthreads();

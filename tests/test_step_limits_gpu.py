@@ -6,6 +6,7 @@ import pytest
 import test_step_gpu as S
 from helpers import bf, f32
 from system1_omni_b200 import lib as L
+from test_step_gpu import up
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +141,34 @@ def test_the_families_status_calls_report_the_steps_codes(cs1, stream, read, wan
     assert getattr(L, read)() == want
     assert getattr(L, read)() == 0
     assert S.status() == ((0, 0, 61) if read == "attn_status" else (0, 31, 0))     # the other family's stays until it is read
+
+
+# ---- large calls ----
+
+def device_us(call, st, n=8):
+    """The quickest of n calls between events."""
+    a, b, us = L.Event(), L.Event(), []
+    for i in range(n + 2):
+        a.record(st)
+        call()
+        b.record(st)
+        st.sync()
+        us.append(a.elapsed_ms(b) * 1e3)
+    return min(us[2:])
+
+
+@pytest.mark.parametrize("nseq", [16384, 65535])
+def test_a_shared_slot_costs_a_large_call_no_more_than_own_ones(cs1, stream, nseq):
+    """The candidates of one prefix: sequences that all begin with one slot, against ones that continue in their own."""
+    kd, vd, H = 8, 16, 1
+    ch = 2 * kd + vd
+    ld = ch + 8
+    x, w, tails = up(bf(np.ones((nseq, ld))), stream), up(bf(np.ones((ch, 4))), stream), up(np.zeros((nseq + 1, 3, ch), np.uint16), stream)
+    al = up(bf(np.ones(8)), stream)
+    q, k, v, beta, g = (L.DeviceBuffer(nseq * 4 * n) for n in (kd, kd, vd, 8, 8))
+    own, one = S.ints(np.arange(nseq), stream), S.ints(np.full(nseq, nseq), stream)
+    times = [device_us(lambda: L.check(cs1.s1_gdn_conv_gates_step(
+        x.at(), ld, w.at(), q.at(), k.at(), v.at(), nseq, kd, vd, x.at(2 * ch), x.at(2 * ch + 2), al.at(), al.at(), beta.at(), g.at(), H, tails.at(),
+        nseq + 1, 3 * ch, None, begin.at(), own.at(), nseq, stream.handle), "step"), stream) for begin in (own, one)]
+    print(nseq, times)
+    assert times[1] < 2 * times[0]
