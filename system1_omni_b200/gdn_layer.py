@@ -85,7 +85,8 @@ class GdnLayer:
     def step(self, x_dev, rows, slot_in, slot_out, nseq, start=None):
         """Queue the layer on new tokens (bf16 [rows, hidden] on the device) that continue sequences: sequence i
         owns rows [start[i], start[i + 1]) (start None: row i) and goes on from slot_in[i] to slot_out[i]; int32
-        arrays on the device, their rules as in s1_gdn_step. The result lands in self.y."""
+        arrays on the device, their rules as in s1_gdn_step. The result lands in self.y; rows without a sequence, or of
+        one that sits out or is refused, come out as zeros."""
         lib, st = self.lib, self.stream.handle
         z = self.proj.at(self.conv * 2)
         b = self.proj.at((self.conv + self.vd) * 2)
@@ -98,6 +99,8 @@ class GdnLayer:
                                            rows, self.kd, self.vd, b, a, self.a_log.at(), self.dt_bias.at(), self.beta.at(), self.g.at(),
                                            self.hv, self.tails.at(), self.slots, 3 * self.conv, start, slot_in, slot_out, nseq, st),
                 "convolution step")
+        # the step leaves the rows that it does not run as they are, which an earlier call filled
+        L.check(lib.s1_memset_async(self.o.at(), 0, rows * self.vd * 2, st), "rows")
         L.check(lib.s1_gdn_step(self.q.at(), self.k.at(), self.v.at(), self.g.at(), self.beta.at(), self.o.at(), rows, self.hv, self.hk,
                                 128 ** -0.5, self.states.at(), self.slots, self.hv * 128 * 128, start, slot_in, slot_out, nseq, st),
                 "delta rule step")

@@ -172,3 +172,40 @@ def test_a_shared_slot_costs_a_large_call_no_more_than_own_ones(cs1, stream, nse
         nseq + 1, 3 * ch, None, begin.at(), own.at(), nseq, stream.handle), "step"), stream) for begin in (own, one)]
     print(nseq, times)
     assert times[1] < 2 * times[0]
+
+
+# ---- the layer ----
+
+def test_layer_rows_that_are_not_run_are_zeros(cs1, stream):
+    """A sequence that sits out, one that is refused and rows that nobody owns show nothing of an earlier call."""
+    from system1_omni_b200.gdn_layer import GdnLayer
+    from test_gdn_layer_gpu import make_case
+    hidden, hk, hv = 256, 1, 4
+    layer = GdnLayer(hidden, hk, hv, max_tokens=64, stream=stream, slots=6)
+    try:
+        x, w = make_case(5, hidden, hk, hv)
+        layer.set_weights(**w)
+        x_dev = up(x, stream)
+        for i in range(5):
+            layer.forward(x_dev.at(i * hidden * 2), 1, slot=i)
+        si = S.ints([0, 1, 2, 3, 4], stream)
+        keep = {n: L.from_device(getattr(layer, n), getattr(layer, n).nbytes, np.uint8, stream) for n in ("states", "tails")}
+        first = S.down(layer.step(x_dev.at(), 5, si.at(), si.at(), 5), (5, hidden), stream)
+        assert (first != 0).any(1).all()
+        for n, a in keep.items():       # the same step again, from the same slots
+            L.check(cs1.cs1_upload(getattr(layer, n).at(), a.ctypes.data, a.nbytes, stream.handle), "upload")
+        so = S.ints([0, -1, 9, 3, 3], stream)                 # goes on, sits out, no such slot, two that write one
+        start = S.ints([0, 1, 2, 3, 4, 5], stream)
+        y = S.down(layer.step(x_dev.at(), 5, si.at(), so.at(), 4, start.at()), (5, hidden), stream)
+        assert S.status()[2] == 61
+        assert (y[0] == first[0]).all() and (y[3] == first[3]).all()
+        assert (y[[1, 2, 4]] == 0).all()
+        y = S.down(layer.step(x_dev.at(), 5, si.at(), so.at(), 5, start.at()), (5, hidden), stream)
+        assert S.status()[2] in (61, 62)
+        assert (y[1:] == 0).all() and (y[0] != 0).any()
+        assert (L.from_device(layer.states, layer.states.nbytes // 6, np.uint8, stream, layer.states.nbytes // 6 * 4) != 0).any()
+        layer.forward(x_dev.at(), 0, slot=4)                  # no tokens: the slot of a sequence that has not begun
+        for buf in (layer.states, layer.tails):
+            assert (L.from_device(buf, buf.nbytes // 6, np.uint8, stream, buf.nbytes // 6 * 4) == 0).all()
+    finally:
+        layer.close()
