@@ -24,6 +24,7 @@ class GdnLayer:
         self.kd, self.vd = k_heads * 128, v_heads * 128
         self.conv = 2 * self.kd + self.vd
         self.gdn_in = self.conv + self.vd + 2 * v_heads
+        self.ld = (self.gdn_in + 7) // 8 * 8  # of a projected row: the step reads it in packs of 8
         self.cap = max_tokens
         self.stream = stream or L.Stream()
         self.gemm = self.lib.cs1_gemm_create(32 << 20)
@@ -33,7 +34,7 @@ class GdnLayer:
         nb = lambda n: L.DeviceBuffer(n)
         self.w_in, self.w_out = nb(self.gdn_in * hidden * 2), nb(hidden * self.vd * 2)
         self.w_conv, self.a_log, self.dt_bias, self.w_norm = nb(self.conv * 4 * 2), nb(v_heads * 2), nb(v_heads * 2), nb(256)
-        self.proj, self.q, self.k, self.v = nb(T * self.gdn_in * 2), nb(T * self.kd * 2), nb(T * self.kd * 2), nb(T * self.vd * 2)
+        self.proj, self.q, self.k, self.v = nb(T * self.ld * 2), nb(T * self.kd * 2), nb(T * self.kd * 2), nb(T * self.vd * 2)
         self.beta, self.g, self.o, self.n = nb(T * v_heads * 2), nb(T * v_heads * 4), nb(T * self.vd * 2), nb(T * self.vd * 2)
         self.ws = nb(self.lib.cs1_gdn_workspace_floats(T, v_heads) * 4)
         self.y = nb(T * hidden * 2)
@@ -67,10 +68,10 @@ class GdnLayer:
         b = self.proj.at((self.conv + self.vd) * 2)
         a = self.proj.at((self.conv + self.vd + self.hv) * 2)
         L.check(lib.cs1_gemm(self.gemm, x_dev, self.w_in.at(), self.proj.at(), T, self.gdn_in, self.hidden,
-                             self.gdn_in, st), "in_proj")
-        L.check(lib.cs1_gdn_conv(self.proj.at(), self.gdn_in, self.w_conv.at(), self.q.at(), self.k.at(), self.v.at(),
+                             self.ld, st), "in_proj")
+        L.check(lib.cs1_gdn_conv(self.proj.at(), self.ld, self.w_conv.at(), self.q.at(), self.k.at(), self.v.at(),
                                  T, self.kd, self.vd, st), "conv")
-        L.check(lib.cs1_gdn_gates(b, a, self.gdn_in, self.a_log.at(), self.dt_bias.at(), self.beta.at(), self.g.at(),
+        L.check(lib.cs1_gdn_gates(b, a, self.ld, self.a_log.at(), self.dt_bias.at(), self.beta.at(), self.g.at(),
                                   T, self.hv, st), "gates")
         L.check(lib.cs1_gdn_prefill_x(self.q.at(), self.k.at(), self.v.at(), self.g.at(), self.beta.at(), self.o.at(),
                                       self.ws.at(), T, self.hv, self.hk, 128 ** -0.5, None, s_out, st), "delta rule")
@@ -78,7 +79,7 @@ class GdnLayer:
             tail, row, kept = slot * 3 * self.conv * 2, self.conv * 2, min(T, 3)
             if kept < 3:    # fewer rows than the convolution looks back: zeros before them
                 L.check(lib.s1_memset_async(self.tails.at(tail), 0, (3 - kept) * row, st), "tail")
-            L.check(lib.cs1_copy2d(self.tails.at(tail + (3 - kept) * row), row, self.proj.at((T - kept) * self.gdn_in * 2), self.gdn_in * 2,
+            L.check(lib.cs1_copy2d(self.tails.at(tail + (3 - kept) * row), row, self.proj.at((T - kept) * self.ld * 2), self.ld * 2,
                                    row, kept, st), "tail")
         return self._output(z, T)
 
@@ -94,8 +95,8 @@ class GdnLayer:
         if rows > self.cap:
             raise ValueError(f"{rows} rows, the layer holds {self.cap}")
         L.check(lib.cs1_gemm(self.gemm, x_dev, self.w_in.at(), self.proj.at(), rows, self.gdn_in, self.hidden,
-                             self.gdn_in, st), "in_proj")
-        L.check(lib.s1_gdn_conv_gates_step(self.proj.at(), self.gdn_in, self.w_conv.at(), self.q.at(), self.k.at(), self.v.at(),
+                             self.ld, st), "in_proj")
+        L.check(lib.s1_gdn_conv_gates_step(self.proj.at(), self.ld, self.w_conv.at(), self.q.at(), self.k.at(), self.v.at(),
                                            rows, self.kd, self.vd, b, a, self.a_log.at(), self.dt_bias.at(), self.beta.at(), self.g.at(),
                                            self.hv, self.tails.at(), self.slots, 3 * self.conv, start, slot_in, slot_out, nseq, st),
                 "convolution step")
@@ -108,7 +109,7 @@ class GdnLayer:
 
     def _output(self, z, T):
         lib, st = self.lib, self.stream.handle
-        L.check(lib.cs1_gated_rms_norm(self.o.at(), z, self.gdn_in, self.w_norm.at(), self.n.at(), T, self.hv, 128,
+        L.check(lib.cs1_gated_rms_norm(self.o.at(), z, self.ld, self.w_norm.at(), self.n.at(), T, self.hv, 128,
                                        self.eps, st), "gated norm")
         L.check(lib.cs1_gemm(self.gemm, self.n.at(), self.w_out.at(), self.y.at(), T, self.hidden, self.vd,
                              self.hidden, st), "out_proj")

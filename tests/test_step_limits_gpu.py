@@ -209,3 +209,24 @@ def test_layer_rows_that_are_not_run_are_zeros(cs1, stream):
             assert (L.from_device(buf, buf.nbytes // 6, np.uint8, stream, buf.nbytes // 6 * 4) == 0).all()
     finally:
         layer.close()
+
+
+@pytest.mark.parametrize("hk,hv", [(1, 1), (1, 2), (3, 3), (2, 6), (5, 5)])
+def test_layer_steps_with_any_number_of_heads(cs1, stream, hk, hv):
+    """Heads whose gates leave a projected row at no multiple of 8: the step takes them as the prefill does."""
+    from system1_omni_b200.gdn_layer import GdnLayer
+    from test_gdn_layer_gpu import make_case, oracle_layer, rel_l2
+    hidden, n, more = 256, 11, 3
+    layer = GdnLayer(hidden, hk, hv, max_tokens=32, stream=stream, slots=1)
+    try:
+        x, w = make_case(n + more, hidden, hk, hv, seed=hv)
+        layer.set_weights(**w)
+        x_dev, slot = up(x, stream), S.ints([0], stream)
+        y = f32(S.down(layer.forward(x_dev.at(), n, slot=0), (32, hidden), stream))[:n]
+        for t in range(more):
+            y = np.concatenate([y, f32(S.down(layer.step(x_dev.at((n + t) * hidden * 2), 1, slot.at(), slot.at(), 1), (1, hidden), stream))])
+        want = f32(oracle_layer(x, w, n + more, hidden, hk, hv, float64_core=True))
+        assert rel_l2(y, want) < 2e-2                          # the gate of the layer's prefill
+        assert np.abs(y - want).max() < 5e-2 * np.abs(want).max()
+    finally:
+        layer.close()
