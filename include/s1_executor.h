@@ -28,8 +28,8 @@ int s1_download_async(void* dst, const void* src, size_t bytes, void* stream);
 int s1_memset_async(void* dst, int value, size_t bytes, void* stream);
 int s1_device_sync(void);
 /* Programmatic dependent launch for the calling host thread's later launches of this library's
- * kernels: mode 1 = every hot-path kernel but the two delta-rule kernels, 2 = the GEMMs and the
- * norms, 0 = plain stream order. A kernel
+ * kernels: mode 1 = every hot-path kernel but the two delta-rule kernels of the prefill, 2 = the GEMMs and the
+ * norms, 0 = plain stream order (the second kernel of s1_attention_paged is a dependent of its first in every mode). A kernel
  * launched so may become resident while the kernel before it on the stream still runs, sets up
  * (the GEMMs also fetch their first weight tiles) and waits for that kernel to complete before it
  * touches activations. Results are the same bits in every mode. Returns the previous mode. The

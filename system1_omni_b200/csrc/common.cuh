@@ -101,6 +101,11 @@ inline cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 // writes - overlaps the kernels before it; the order of all other memory effects is that of
 // ordinary stream order, since grid_dep_sync() returns only when the kernel before is complete
 // and its writes are visible, and that kernel in turn waited for the one before it.
+// One pair of kernels departs from this: the paged attention's join is a dependent of the kernel before it in every
+// mode, and reads the rows' sequences and lengths before its grid_dep_sync(). That is sound because the
+// attention's first kernel calls grid_dep_trigger() only behind its own grid_dep_sync(), when whatever wrote them is
+// complete, because it does not write them itself, and because the join reads them past L1. Moved to the top, where the
+// other kernels have it, the trigger would let the join cut by lengths of the step before.
 // The switch is per host thread and has three settings: nearly every hot-path kernel (the
 // executor's choice for short prompts issued eagerly, where launch gaps, prologues and the first
 // trip to HBM are a large part of every kernel), the GEMMs and the norms after them (its choice
@@ -111,7 +116,8 @@ inline cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 __device__ __forceinline__ void grid_dep_sync() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// The switch: 0 = plain stream order, 1 = every hot-path kernel but the delta-rule pair, 2 = the GEMMs and norms.
+// The switch: 0 = plain stream order (but for the paged attention's join), 1 = every hot-path kernel but the prefill's delta-rule
+// pair, 2 = the GEMMs and norms.
 inline int& dep_launch_switch() {
     static thread_local int mode = 0;
     return mode;
@@ -120,7 +126,7 @@ inline int& dep_launch_switch() {
 inline int dep_launch_mode() { return dep_launch_switch(); }
 // Kernel families, for the choice of which launches become dependents.
 enum DepFamily { DEP_GEMM = 1, DEP_GDN = 2, DEP_ATTENTION = 4, DEP_NORM = 8, DEP_OTHER = 16 };
-// What the two modes cover, from measurements on the 4B-shaped decoder: the delta-rule kernels are
+// What the two modes cover, from measurements on the 4B-shaped decoder: the prefill's delta-rule kernels are
 // never launched as dependents (their blocks take most of an SM's shared memory while they wait:
 // -4 % at 1024 tokens, and short passes are faster without them too); mode 1 takes everything
 // else, mode 2 the GEMMs and the norms that follow them.

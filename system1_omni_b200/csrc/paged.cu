@@ -402,7 +402,6 @@ __device__ __forceinline__ long long row_tiles(const PagedArgs& a, const uint32_
 struct Cut {
     long long total;
     int runs;
-    Cut() = default;
     __device__ Cut(long long t, int blocks, long long pieces)
         : total(t), runs((int)min((long long)blocks, min(t, max((t + RUN - 1) / RUN, PARTS * pieces)))) {}
     // (up to 2^22 tiles, 67 million tokens, in 32 bits, whose division is shorter)
@@ -508,7 +507,7 @@ __global__ void __launch_bounds__(PAGED_THREADS, PCfg<DH>::BLOCKS_PER_SM)
         prefetch_tmap(&maps.v);
     }
     grid_dep_sync();
-    grid_dep_trigger();  // not before: the join reads the lengths without a wait of its own
+    grid_dep_trigger();  // not before: the join reads sequences and lengths without a wait of its own
 
     // ---- this block's run of the line of tiles ----
     if constexpr (WINDOWS) find_windows<false, PAGED_THREADS>(a, on);
