@@ -136,8 +136,8 @@ int s1_gdn_conv_gates_step(const void* qkv, int ld, const void* w, void* q, void
                            const int* slot_in, const int* slot_out, int nseq, void* stream);
 
 /* A paged cache of one full-attention layer: two pools [n_pages, page_tokens, Hk, Dh] (keys after norm
- * and rotary, values as projected; a captured prefix's keys are such a pool where page_tokens divides
- * its length) and a table [n_seqs, table_pages] of page numbers: token p of sequence s is row
+ * and rotary, values as projected; the keys that cs1_attn_prep leaves for T tokens are such a pool of T / page_tokens pages
+ * where that divides, their values once cs1_copy2d has taken them out of the projection's rows) and a table [n_seqs, table_pages] of page numbers: token p of sequence s is row
  * p % page_tokens of page table[s][p / page_tokens]. Entries behind a sequence's last page are never
  * read; sequences may share pages. n_pages * page_tokens < 2^31, table_pages * page_tokens <= 2^30.
  *
@@ -156,8 +156,10 @@ int s1_attn_prep_paged(const void* qg, const void* kr, const void* vr, int ld, c
 /* Attention of one new token per row: q, out [rows, Hq, Dh], row r over the first len[r] tokens of
  * sequence seq[r] (null: r), its own one among them; several rows of one sequence with growing len
  * are a causal window. Neighbouring rows of a window, each at most 16 tokens longer than the one before, read a
- * large cache once for as many of them as have 16 query heads per key-value head together, in calls with
- * more rows than sequences and at most 8192 rows. gate (nullable) [rows, Hq, Dh]: out = o * sigmoid(gate). len 0:
+ * large cache once for as many of them (w) as have 16 query heads per key-value head together, in calls with
+ * more rows than n_seqs and at most 8192 rows, whose table could hold 64 MB / (w - 1) of keys and values: its size decides
+ * (n_seqs * table_pages pages), since the lengths are on the device, so pass the rows of the step's sequences alone and no wider
+ * than the longest may become. Where w is 1, nothing is shared. gate (nullable) [rows, Hq, Dh]: out = o * sigmoid(gate). len 0:
  * zeros; len negative: the row sits out, out is left as it is. A row with a page outside the pools comes out
  * undefined (code 32), a row that the table does not have is left as it is (code 31); a row whose scores
  * are all -inf comes out as zeros. page_tokens a multiple of 16, Dh 128 or 256, Hq a multiple of Hk, at

@@ -47,7 +47,9 @@ class Pages:
         return self.lib.s1_pages_free_count(self.handle)
 
     def table(self, seq=0, n=None):
-        """(page table [n, max_seq_pages], tokens [n]) of the sequences from `seq` on, int32."""
+        """(page table [n, max_seq_pages], tokens [n]) of the sequences from `seq` on, int32. s1_attention_paged goes by the
+        table's size (whether there are windows, and how large the caches may be): give it the rows of a step's sequences,
+        and the columns that the longest of them may come to fill."""
         n = self.max_seqs - seq if n is None else n
         table, tokens = np.empty((n, self.max_seq_pages), np.int32), np.empty(n, np.int32)
         L.check(self.lib.s1_pages_table(self.handle, seq, n, table.ctypes.data, self.max_seq_pages, tokens.ctypes.data), "pages table")
