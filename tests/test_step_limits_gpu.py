@@ -230,3 +230,103 @@ def test_layer_steps_with_any_number_of_heads(cs1, stream, hk, hv):
         assert np.abs(y - want).max() < 5e-2 * np.abs(want).max()
     finally:
         layer.close()
+
+
+# ---- groups at their limits ----
+
+@pytest.mark.parametrize("hurt", [False, True])
+def test_convolution_of_the_most_sequences(cs1, stream, hurt):
+    """65535 sequences, 127 to a block, the last block short."""
+    S.test_convolution_step_of_many_sequences(cs1, stream, 65535, hurt)
+
+
+@pytest.mark.parametrize("hurt", [False, True])
+def test_prep_of_the_most_rows(cs1, stream, hurt):
+    """65536 rows, 128 to a block."""
+    S.test_prep_of_many_rows(cs1, stream, 65536, 128, 2, 1, 48, hurt)
+
+
+@pytest.mark.parametrize("nseq,H,HK,per", [(65535, 9, 3, 128), (43000, 16, 8, 128), (3000, 6, 6, 4)])
+@pytest.mark.parametrize("hurt", [False, True])
+def test_delta_rule_with_the_most_sequences_to_a_block(cs1, stream, nseq, H, HK, per, hurt):
+    """Sequences that sit out, but for some: scattered, and every one of a block; all rows against the formula."""
+    assert min(128, nseq * H // 4096) == per
+    rng = np.random.default_rng(nseq + hurt)
+    block = per * (nseq // per // 2)
+    live = np.unique(np.concatenate([rng.permutation(nseq)[:60], block + np.arange(per), [0, per - 1, per, nseq - 1]]))
+    lens = np.zeros(nseq, int)
+    lens[live] = rng.integers(0, 4, len(live))
+    lens[rng.permutation(nseq)[:50]] = 1                          # rows of sequences that sit out
+    start = np.concatenate([[0], np.cumsum(lens)])
+    so, si = np.full(nseq, -1), rng.integers(-1, 300, nseq)       # what begins a sequence that sits out is nobody's matter
+    n = len(live)
+    slots = n + 2
+    so[live] = rng.permutation(n)
+    si[live] = np.where(rng.random(n) < 0.4, n, np.where(rng.random(n) < 0.5, so[live], -1))
+    refused = np.zeros(nseq, bool)
+    if hurt:
+        a, b, c, d, e = live[rng.permutation(n)[:5]]
+        so[a] = so[b]                                             # two write one slot
+        si[c], si[d] = so[d], -1                                  # one begins with what another writes
+        so[e] = slots                                             # no such slot
+        for i in live:
+            others = [j for j in live if j != i]
+            refused[i] = so[i] >= slots or any(so[i] in (so[j], si[j]) or (si[i] >= 0 and si[i] == so[j]) for j in others)
+        assert refused[[a, b, c, d, e]].all() and refused.sum() < 12
+    x = S.delta_inputs(start[-1], H, HK, slots, nseq)
+    w, states, tol, tol_s = S.delta_formula(x, start, si, np.where(refused, -1, so), H, HK, S.D ** -0.5)
+    got, new = S.run_delta(cs1, stream, x, start, si, so, H, HK, S.D ** -0.5, fill=int(NAN))
+    assert (S.status()[2] in (61, 62)) == hurt
+    rest = np.isnan(w)
+    assert (got[rest] == NAN).all() and np.isfinite(f32(got[~rest])).all()
+    assert (np.abs(f32(got).astype(np.float64) - w)[~rest] <= tol[~rest]).all()
+    assert (np.abs(new.astype(np.float64) - states) <= tol_s).all()
+
+
+@pytest.mark.parametrize("nseq", [2561, 9001])
+def test_delta_rule_of_many_sequences_writes_every_row(cs1, stream, nseq):
+    H, HK, scale = 4, 2, S.D ** -0.5
+    x = S.delta_inputs(nseq, H, HK, 1, nseq)
+    pool = L.DeviceBuffer(nseq * H * S.D * S.D * 4)
+    d = {m: up(x[m], stream) for m in ("q", "k", "v", "g", "beta")}
+    o = up(np.full(x["v"].shape, NAN, np.uint16), stream)
+    so, si = S.ints(np.random.default_rng(1).permutation(nseq), stream), S.ints(np.full(nseq, -1), stream)
+    L.check(cs1.s1_gdn_step(d["q"].at(), d["k"].at(), d["v"].at(), d["g"].at(), d["beta"].at(), o.at(), nseq, H, HK, scale, pool.at(), nseq,
+                            H * S.D * S.D, None, si.at(), so.at(), nseq, stream.handle), "step")
+    got = f32(S.down(o, x["v"].shape, stream)).astype(np.float64)
+    # from zeros: S = k (beta v)^T, o = (q.k) beta v
+    q, k, v, beta = (f32(x[m]).astype(np.float64) for m in ("q", "k", "v", "beta"))
+    q, k = (a / np.sqrt((a ** 2).sum(-1, keepdims=True) + 1e-6) for a in (q, k))
+    head = np.arange(H) // (H // HK)
+    want = ((q * k).sum(-1) * scale)[:, head, None] * beta[..., None] * v
+    # q.k is a sum of 128 products of unit vectors (48 roundings as in delta_formula), the rest a few more
+    tol = HALF * np.abs(want) + 96 * EPS * scale * beta[..., None] * np.abs(v)
+    assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("nseq,H,HK,tokens", [(40, 16, 8, 2), (4100, 4, 2, 1)])
+def test_dependent_launches_of_wide_and_grouped_steps_give_the_same_bits(cs1, stream, nseq, H, HK, tokens):
+    """Convolution and delta rule in a chain, in place, with four warps to a block and with several sequences to one."""
+    rows = nseq * tokens
+    kd, vd = HK * S.D, H * S.D
+    c = S.conv_case(rows, kd, vd, H, nseq, 0, 6)
+    start = None if tokens == 1 else S.ints(np.arange(nseq + 1) * tokens, stream)
+    res = []
+    for mode in (0, 1, 2):
+        before = cs1.s1_set_dependent_launch(mode)
+        cd = {k: up(c[k], stream) for k in ("x", "w", "al", "dt", "tails")}
+        q, k, v, o = (L.DeviceBuffer(rows * w * 2) for w in (kd, kd, vd, vd))
+        beta, g, states = L.DeviceBuffer(rows * H * 2), L.DeviceBuffer(rows * H * 4), L.DeviceBuffer(nseq * H * S.D * S.D * 4)
+        L.check(cs1.s1_memset_async(states.at(), 0, states.nbytes, stream.handle), "memset")
+        s = S.ints(np.arange(nseq), stream)
+        for _ in range(6):
+            L.check(cs1.s1_gdn_conv_gates_step(cd["x"].at(), c["ld"], cd["w"].at(), q.at(), k.at(), v.at(), rows, kd, vd, cd["x"].at(2 * c["ch"]),
+                                               cd["x"].at(2 * (c["ch"] + H)), cd["al"].at(), cd["dt"].at(), beta.at(), g.at(), H, cd["tails"].at(),
+                                               nseq, 3 * c["ch"], S.at(start), s.at(), s.at(), nseq, stream.handle), "conv")
+            L.check(cs1.s1_gdn_step(q.at(), k.at(), v.at(), g.at(), beta.at(), o.at(), rows, H, HK, S.D ** -0.5, states.at(), nseq, H * S.D * S.D,
+                                    S.at(start), s.at(), s.at(), nseq, stream.handle), "step")
+        cs1.s1_set_dependent_launch(before)
+        res.append((S.down(o, (rows, vd), stream), S.down(states, (nseq * H * S.D * S.D,), stream, np.float32)))
+    assert np.isfinite(f32(res[0][0])).all() and np.abs(res[0][1]).max() > 0
+    for other in res[1:]:
+        assert (other[0] == res[0][0]).all() and (other[1] == res[0][1]).all()
