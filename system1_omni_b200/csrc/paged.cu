@@ -279,8 +279,8 @@ __global__ void __launch_bounds__(PREP_THREADS) attn_prep_paged_many_kernel(cons
 //
 // Measured, in a recorded graph: 65 caches of 500 to 16000 tokens, 24 query and 4 key-value heads of 128
 // (630 MB): 102 us, 6.2 TB/s with the join; 250001 tokens, 16 and 4 heads of 256 (1.02 GB): 160 us, 6.4 TB/s;
-// 1500 tokens: 8.3 us; 3 rows of 2 tokens: 7.6. Without the join: 97, 150, 5.5 and 6.5, the first kernel at the rate of a
-// copy. Before, tiles of 64 tokens of one head whose warps shared every tile's maximum and probabilities: 119 us (one
+// 1500 tokens: 8.3 us; 3 rows of 2 tokens: 7.6. The join takes 5.6, 5.2, 2.9 and 1.5 of these, so the first kernel runs at
+// the rate of a copy. Before, tiles of 64 tokens of one head whose warps shared every tile's maximum and probabilities: 119 us (one
 // block per SM), 113 (two) for the first.
 constexpr int CONSUMERS = 4, PAGED_THREADS = (CONSUMERS + 1) * 32;
 constexpr int SLICE = 16;       // tokens of a warp's part of a tile, and of a copied box

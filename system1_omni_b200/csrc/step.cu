@@ -370,7 +370,7 @@ extern "C" int s1_gdn_step(const void* q, const void* k, const void* v, const fl
     const int rc = error_word(&error);
     if (rc != 0) return rc;
     // Many sequences: several to a block, which looks all others up at once, where every block would compare all with
-    // one. 4 heads, one to a block and several: 2048 sequences 183 and 199 us, 4096: 437 and 401, 16384: 3.5 and 1.7 ms.
+    // one. 4 heads, one to a block and several: 2048 sequences 183 and 199 us, 4096: 437 and 396, 16384: 3.5 and 1.6 ms.
     const int per = nseq > MANY_SEQS ? (int)std::min<long long>(STEP_ROWS, heads / 4096) : 1;
     const bool many = per > 1;
     const long long blocks = few ? 4 * heads : many ? (long long)((nseq + per - 1) / per) * H : heads;
@@ -402,7 +402,9 @@ extern "C" int s1_gdn_conv_gates_step(const void* qkv, int ld, const void* w, vo
     if (rc != 0) return rc;
     const int conv_blocks = (channels / 8 + CONV_THREADS - 1) / CONV_THREADS;
     // Several sequences to a block as in s1_gdn_step. 10240 channels, one to a block and several: 1500 sequences 55 and 68 us,
-    // 4096: 181 and 165; 1536 channels, 16384: 480 and 206 us, 65535: 11.2 and 1.05 ms.
+    // 4096: 181 and 162; 1536 channels, 16384: 480 and 174 us, 65535: 11.2 and 0.68 ms (the bytes alone 61 and 245), whether
+    // they begin in slots of their own or in one. What is left beside the bytes: every block reads all slots, and a thread has one
+    // sequence's rows in flight.
     const int per = nseq >= CONV_MANY ? std::min(STEP_ROWS, nseq / 512) : 1;
     const cudaError_t e = launch_dep(
         per > 1 ? gdn_conv_gates_step_kernel<true> : gdn_conv_gates_step_kernel<false>, dim3(conv_blocks + 1, (nseq + per - 1) / per),
