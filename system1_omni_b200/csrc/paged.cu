@@ -447,7 +447,8 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Two probabilities as two bf16 terms each, hi + lo within 2^-15 of p: hi is p (1 - 2^-16) cut to its upper half,
-// which lies below p wherever p > 0, so that lo > 0 too and both products with an infinite value have its sign.
+// which lies below p wherever p > 0, so that lo > 0 too and both products with an infinite value have its sign (with p
+// above 2^-117; below, lo may be zero in bf16).
 __device__ __forceinline__ void two_terms(float p0, float p1, uint32_t& hi, uint32_t& lo) {
     const uint32_t h0 = __float_as_uint(p0 * 0.9999847412109375f), h1 = __float_as_uint(p1 * 0.9999847412109375f);
     hi = __byte_perm(h0, h1, 0x7632);

@@ -73,7 +73,7 @@ def test_probabilities_of_a_window_enter_the_product_as_float32(cs1, stream, Dh,
 @pytest.mark.parametrize("equal", [True, False])
 @pytest.mark.parametrize("window", [True, False])
 def test_infinite_values_keep_their_sign(cs1, stream, Dh, Hq, Hk, equal, window):
-    """An infinite value of a token that a row sees makes that dim infinite, whatever the token's weight, and no other dim."""
+    """An infinite value of a token that a row sees makes that dim infinite, whichever weight the token has, and no other dim."""
     lens, seq = S.windows_of([(0, 40, 4, 1), (1, 1, 1, 0), (2, 100, 3, 1)])
     c = S.attn_case(lens, Hq, Hk, Dh, 16, 8, seq=seq)
     if equal:
