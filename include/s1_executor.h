@@ -104,7 +104,8 @@ int s1_gdn_conv_gates_batch(const void* qkv, int ld, const void* w, void* q, voi
  * (slots, positions, lengths, page tables) is int32 in device memory, so a recorded step replays with
  * new contents; the kernels check every index before they use it. What they refuse they leave
  * unwritten, with a code in a device error word of the family's step operators: 60 rows outside the
- * operands or out of order (rows that two other sequences then share hold either's result), 61 a slot outside the pool, 62 sequences that would race for a slot (delta-rule family);
+ * operands or out of order (rows that two other sequences then share hold either's result), 61 a slot outside
+ * the pool, 62 sequences that would race for a slot (delta-rule family);
  * 31 a row whose sequence or position the table does not have, 32 a page outside the pools, 33 a
  * position outside the rotary tables, 34 rows at one place of the cache, 30 a bounded wait that ran out
  * (attention family). A code stays until s1_device_status, s1_gdn_status or s1_attn_tc5_status reads it; the
